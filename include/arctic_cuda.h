@@ -168,6 +168,57 @@ int ae_get_attention_mode(const ae_ctx* ctx);
 int ae_attention_i8(ae_ctx* ctx, const float* d_qkv, const uint32_t* d_cu_seqlens, uint32_t n_seqs,
                     uint32_t max_len, float* d_ctx);
 
+/* ---------------------------------------------------------------------------------------------
+ * Layers of other encoders and decoders next to this model's own: the int8 product in general form, and
+ * the norm and rotation of queries and keys (no counterpart in the reference, whose product is tied to its
+ * packed weights and whose positions are learned). Device buffers, asynchronous on the context's stream.
+ * They need no loaded model. Float operands and results are of type: */
+enum { AE_F32 = 0, AE_F16 = 1, AE_BF16 = 2 };
+
+/* Product of int8 activations, with a scale for each token, and int8 weights, with a scale for each
+ * output channel:
+ *   out[m, n] = fma(float(sum_k a[m, k] w[n, k]), a_scale[m] * w_scale[n], bias[n])
+ * a [M, K], w [N, K] (out_features x in_features), a_scale [M], w_scale [N], bias [N] or NULL (zeros), out
+ * [M, N] of out_type. The sum is exact (int32, hence K <= 131,071); the result is rounded to out_type once.
+ * lda, ldw (bytes) and ldo (elements) are the rows' pitches, at least the rows' lengths. Any M (0: nothing
+ * is done), N and K. Operands that start on 16 bytes with a pitch that is a multiple of 16 are read where
+ * they are; others are first laid out so in scratch that the context keeps for each stream (grown on
+ * demand, which synchronises the stream; run once before a stream capture). out overlaps no operand. */
+int ae_matmul_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_a, uint64_t lda,
+                 const float* d_a_scale, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
+                 const float* d_bias, int out_type, void* d_out, uint64_t ldo);
+
+/* The same product from float activations x [M, K] of x_type (row pitch ldx elements), quantized per
+ * token on the way as the model's own SmoothQuant rows are (smooth_quantize_row, src/simd_math.rs:584-649):
+ *   y = x * inv_smooth (NULL: ones);  top = max_k |y|;  a = round_half_even(y * (127 / top));
+ *   a_scale = top / 127
+ * A token whose top is below 2^-119 (127 / top would not be finite) quantizes to zeros with a scale of 0;
+ * one that holds an infinity or a NaN gives a row of NaN. */
+int ae_linear_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, int x_type, const void* d_x, uint64_t ldx,
+                 const float* d_inv_smooth, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
+                 const float* d_bias, int out_type, void* d_out, uint64_t ldo);
+
+/* RMS norm of every query and key head, and the rotation of its first rotary_dim dims by the token's
+ * position, in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * weight;  (y_i, y_j) -> (y_i c - y_j s, y_j c + y_i s)
+ * computed in float and rounded to `type` once. Pairs (i, i + rotary_dim / 2), or with AE_QK_NEIGHBOURS
+ * (2i, 2i + 1); AE_QK_NO_NORM leaves the norm (and the weights) out. head_dim 1..512, rotary_dim even and
+ * 0..head_dim. Element i of head h of token t lies at t * token_stride + h * head_stride + i (elements), so
+ * heads are read and written where a packed projection has them; outputs may be the inputs themselves
+ * (same address and strides), and overlap nothing otherwise. weights [head_dim] or NULL (ones).
+ * table [table_rows, rotary_dim] f32: row p holds the cosines of position p's rotary_dim / 2 angles, then
+ * their sines. A token's position is d_positions[t], or, where that is NULL, its place in its sequence
+ * (rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 of n_seqs sequences). A position outside the table is
+ * reported as AE_ERR_DEVICE by ae_sync, and its token's outputs are not written. */
+enum { AE_QK_NEIGHBOURS = 1, AE_QK_NO_NORM = 2 };
+int ae_qk_norm_rope(ae_ctx* ctx, int type, uint32_t tokens, uint32_t q_heads, uint32_t k_heads, uint32_t head_dim,
+                    uint32_t rotary_dim, int flags, const void* d_q, uint64_t q_token_stride,
+                    uint64_t q_head_stride, const void* d_k, uint64_t k_token_stride, uint64_t k_head_stride,
+                    void* d_q_out, uint64_t q_out_token_stride, uint64_t q_out_head_stride, void* d_k_out,
+                    uint64_t k_out_token_stride, uint64_t k_out_head_stride, const float* d_q_weight,
+                    const float* d_k_weight, float eps, const float* d_table, uint32_t table_rows,
+                    const int32_t* d_positions, const uint32_t* d_cu_seqlens, uint32_t n_seqs);
+
 /* Allocation-free variant of the single-sequence forward, for callers that cannot call cudaMalloc
  * when they embed: hosts that hand out device memory once at start-up from their own pool (a
  * service with a fixed memory budget), and latency paths that must not block on the allocator

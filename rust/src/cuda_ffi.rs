@@ -19,6 +19,13 @@ pub const AE_ERR_CAPACITY: c_int = -7;
 pub const AE_ATTENTION_EXACT: c_int = 0;
 pub const AE_ATTENTION_INT8: c_int = 1;
 
+pub const AE_F32: c_int = 0;
+pub const AE_F16: c_int = 1;
+pub const AE_BF16: c_int = 2;
+
+pub const AE_QK_NEIGHBOURS: c_int = 1;
+pub const AE_QK_NO_NORM: c_int = 2;
+
 pub const AE_TRACE_EMBED: c_int = 0;
 pub const AE_TRACE_ATTN0: c_int = 1;
 
@@ -107,6 +114,20 @@ extern "C" {
     pub fn ae_get_attention_mode(ctx: *const ae_ctx) -> c_int;
     pub fn ae_attention_i8(ctx: *mut ae_ctx, d_qkv: *const f32, d_cu_seqlens: *const u32, n_seqs: u32,
                            max_len: u32, d_ctx: *mut f32) -> c_int;
+    pub fn ae_matmul_i8(ctx: *mut ae_ctx, m: u32, n: u32, k: u32, d_a: *const i8, lda: u64, d_a_scale: *const f32,
+                        d_w: *const i8, ldw: u64, d_w_scale: *const f32, d_bias: *const f32, out_type: c_int,
+                        d_out: *mut c_void, ldo: u64) -> c_int;
+    pub fn ae_linear_i8(ctx: *mut ae_ctx, m: u32, n: u32, k: u32, x_type: c_int, d_x: *const c_void, ldx: u64,
+                        d_inv_smooth: *const f32, d_w: *const i8, ldw: u64, d_w_scale: *const f32,
+                        d_bias: *const f32, out_type: c_int, d_out: *mut c_void, ldo: u64) -> c_int;
+    pub fn ae_qk_norm_rope(ctx: *mut ae_ctx, dtype: c_int, tokens: u32, q_heads: u32, k_heads: u32, head_dim: u32,
+                           rotary_dim: u32, flags: c_int, d_q: *const c_void, q_token_stride: u64,
+                           q_head_stride: u64, d_k: *const c_void, k_token_stride: u64, k_head_stride: u64,
+                           d_q_out: *mut c_void, q_out_token_stride: u64, q_out_head_stride: u64,
+                           d_k_out: *mut c_void, k_out_token_stride: u64, k_out_head_stride: u64,
+                           d_q_weight: *const f32, d_k_weight: *const f32, eps: f32, d_table: *const f32,
+                           table_rows: u32, d_positions: *const i32, d_cu_seqlens: *const u32, n_seqs: u32)
+        -> c_int;
     pub fn ae_forward_cls_noalloc(ctx: *mut ae_ctx, d_ids: *const u16, len: u32, d_out384: *mut f32) -> c_int;
     pub fn ae_trace_forward(ctx: *mut ae_ctx, ids: *const u16, cu_seqlens: *const u32, n_seqs: u32, stage: c_int,
                             f32_rows: *mut f32, q: *mut i8, scale: *mut f32) -> c_int;

@@ -26,7 +26,7 @@ ATTENTION_EXACT, ATTENTION_INT8 = 0, 1
 
 __all__ = [
     "AeError", "Engine", "ArcticEmbedS", "Workspace", "ParallelContext", "cosine_similarity", "default_model_dir",
-    "embed_batch_multi", "pack_sequences", "plan_shards", "HIDDEN_SIZE", "ATTENTION_EXACT", "ATTENTION_INT8",
+    "embed_batch_multi", "pack_sequences", "plan_shards", "rope_table", "HIDDEN_SIZE", "ATTENTION_EXACT", "ATTENTION_INT8",
 ]
 
 
@@ -51,6 +51,35 @@ def _ptr(a) -> int | None:
         assert a.flags["C_CONTIGUOUS"], "array must be C-contiguous"
         return a.ctypes.data
     return a.data_ptr()  # torch tensor (device memory)
+
+
+# element types of the general operators' float tensors (AE_F32 / AE_F16 / AE_BF16)
+_FLOAT_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
+def _float_type(t, what: str) -> int:
+    code = _FLOAT_TYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def _operand(t, what: str, shape: tuple, dtype: str, device: int):
+    """A tensor of this shape and type in device memory of GPU `device`, its last axis contiguous."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what} must be {shape}, not {tuple(t.shape)}")
+    if dtype is not None and str(t.dtype) != dtype:
+        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{what} must be in device memory of GPU {device}")
+    if t.stride(-1) != 1 and shape[-1] > 1 and t.numel():
+        raise ValueError(f"{what} must be contiguous along its last axis")
+    return t.data_ptr()
+
+
+def _pitch(t) -> int:
+    """Row pitch of a 2-D tensor in elements; that of a single row is the row's own length."""
+    return t.stride(0) if t.shape[0] > 1 and t.shape[1] else t.shape[1]
 
 
 def _linear_desc(lin: ae8.QuantizedLinear | None, keep: list) -> LinearDesc:
@@ -193,6 +222,73 @@ class Engine:
         """ae_attention_i8: the reference's int8 attention scheme on device buffers (every sequence)."""
         self._check(lib().ae_attention_i8(self._h, _ptr(qkv), _ptr(cu), n_seqs, max_len, _ptr(ctx)))
 
+    def _weights(self, w, w_scale, bias, out, M: int):
+        """The checks and arguments matmul_i8 and linear_i8 share."""
+        if w.dim() != 2:
+            raise ValueError("w must be [out_features, in_features]")
+        N, K = w.shape
+        dev = self.device
+        return (N, K, (_operand(w, "w", (N, K), "torch.int8", dev), _pitch(w),
+                       _operand(w_scale, "w_scale", (N,), "torch.float32", dev),
+                       None if bias is None else _operand(bias, "bias", (N,), "torch.float32", dev)),
+                (_float_type(out, "out"), _operand(out, "out", (M, N), None, dev), _pitch(out)))
+
+    def matmul_i8(self, a, a_scale, w, w_scale, out, bias=None) -> None:
+        """ae_matmul_i8: out[m, n] = (sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n]) + bias[n] on device
+        tensors: a [M, K] and w [N, K] int8, a_scale [M], w_scale [N] and bias [N] float32, out [M, N]
+        float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream."""
+        M = a.shape[0]
+        N, K, weights, result = self._weights(w, w_scale, bias, out, M)
+        self._check(lib().ae_matmul_i8(self._h, M, N, K, _operand(a, "a", (M, K), "torch.int8", self.device),
+                                       _pitch(a),
+                                       _operand(a_scale, "a_scale", (M,), "torch.float32", self.device), *weights,
+                                       *result))
+
+    def linear_i8(self, x, w, w_scale, out, bias=None, inv_smooth=None) -> None:
+        """ae_linear_i8: the same product from float activations x [M, K] (float32, float16 or bfloat16),
+        multiplied by inv_smooth [K] and quantized to int8 with a scale for each token on the way."""
+        M = x.shape[0]
+        N, K, weights, result = self._weights(w, w_scale, bias, out, M)
+        dev = self.device
+        smooth = None if inv_smooth is None else _operand(inv_smooth, "inv_smooth", (K,), "torch.float32", dev)
+        self._check(lib().ae_linear_i8(self._h, M, N, K, _float_type(x, "x"), _operand(x, "x", (M, K), None, dev),
+                                       _pitch(x), smooth, *weights, *result))
+
+    QK_NEIGHBOURS, QK_NO_NORM = 1, 2
+
+    def qk_norm_rope(self, q, k, q_out, k_out, table=None, positions=None, cu=None, q_weight=None, k_weight=None,
+                     eps: float = 1e-6, neighbours: bool = False, norm: bool = True) -> None:
+        """ae_qk_norm_rope: RMS norm (q_weight, k_weight [dim] float32) of the heads q [T, q_heads, dim] and
+        k [T, k_heads, dim] and the rotation of their first table.shape[1] dims, into q_out and k_out (which
+        may be q and k). table [rows, rotary] float32 is rope_table's; a token's position is positions[t]
+        (int32), or its place in its sequence of cu (int32 or uint32 [n_seqs + 1])."""
+        T, Hq, D = q.shape
+        Hk, dev, dt, code = k.shape[1], self.device, str(q.dtype), _float_type(q, "q")
+        heads = ()
+        for t, what, H in ((q, "q", Hq), (k, "k", Hk), (q_out, "q_out", Hq), (k_out, "k_out", Hk)):
+            heads += (_operand(t, what, (T, H, D), dt, dev), t.stride(0), t.stride(1))
+        rows = rotary = n_seqs = 0
+        tp = pp = cp = None
+        if table is not None:
+            rows, rotary = table.shape
+            if not table.is_contiguous():
+                raise ValueError("table must be contiguous")
+            tp = _operand(table, "table", (rows, rotary), "torch.float32", dev)
+            if positions is not None:
+                pp = _operand(positions, "positions", (T,), "torch.int32", dev)
+            elif cu is not None:
+                n_seqs = len(cu) - 1
+                if str(cu.dtype) not in ("torch.int32", "torch.uint32"):
+                    raise ValueError(f"cu must be int32 or uint32, not {cu.dtype}")
+                cp = _operand(cu, "cu", (n_seqs + 1,), None, dev)
+            else:
+                raise ValueError("a rotation needs positions or cu")
+        qw = None if q_weight is None else _operand(q_weight, "q_weight", (D,), "torch.float32", dev)
+        kw = None if k_weight is None else _operand(k_weight, "k_weight", (D,), "torch.float32", dev)
+        flags = (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM)
+        self._check(lib().ae_qk_norm_rope(self._h, code, T, Hq, Hk, D, rotary, flags, *heads, qw, kw, eps, tp, rows,
+                                          pp, cp, n_seqs))
+
     def set_attention_mode(self, mode: int) -> "Engine":
         """ATTENTION_EXACT (fp32, default) or ATTENTION_INT8 (the reference's int8 scheme) for layers 0-10."""
         self._check(lib().ae_set_attention_mode(self._h, int(mode)))
@@ -252,6 +348,13 @@ def plan_shards(cu: np.ndarray, n_shards: int) -> np.ndarray:
     if code != 0:
         raise AeError(code, "ae_plan_shards: invalid arguments")
     return out
+
+
+def rope_table(rows: int, rotary_dim: int, base: float = 10000.0) -> np.ndarray:
+    """Rotation table of positions 0 .. rows - 1 for Engine.qk_norm_rope, float32 [rows, rotary_dim]: the
+    cosines, then the sines, of p * base^(-2i / rotary_dim), the angles in float64."""
+    angle = np.outer(np.arange(rows, dtype=np.float64), base ** (-np.arange(0, rotary_dim, 2) / rotary_dim))
+    return np.concatenate([np.cos(angle), np.sin(angle)], axis=1).astype(np.float32)
 
 
 class Workspace:

@@ -37,6 +37,7 @@
 #include "gemm_i8.h"
 #include "kernels.h"
 #include "latency.h"
+#include "linear_i8.h"
 #include "ptx.cuh"
 #include "rowmath.cuh"
 
@@ -122,6 +123,13 @@ struct ae_ctx {
   uint32_t* d_cu_single = nullptr;  // [513][2]: {0, L} at 2L, the cu_seqlens of one sequence of L ids
   float* d_gemm_scratch = nullptr;  // ae_gemm_i8's split LayerNorm path: h of up to gemm_scratch_rows rows
   uint32_t gemm_scratch_rows = 0;
+  // scratch of ae_matmul_i8 / ae_linear_i8, one for each stream the context was set to, so that a call
+  // on one stream never writes what a call on another may still be reading
+  struct Scratch {
+    uint8_t* p = nullptr;
+    size_t bytes = 0;
+  };
+  std::map<cudaStream_t, Scratch> scratch;
   bool has_model = false;
   DevModel model;
   void* h_model = nullptr;  // pinned host image of the model arena (reused across loads)
@@ -726,8 +734,9 @@ int enqueue_forward(ae_ctx* c, const uint16_t* d_ids, const uint32_t* d_cu, int 
 
 int dev_err_fail(ae_ctx* c, int h) {
   static const char* names[] = {"ok", "producer wait timed out", "MMA wait timed out", "epilogue wait timed out",
-                                "sequence length outside 1..512", "token id out of range"};
-  return fail(c, AE_ERR_DEVICE, "device error %d (%s)", h, (h >= 0 && h <= 5) ? names[h] : "?");
+                                "sequence length outside 1..512", "token id out of range",
+                                "position outside the rotation table"};
+  return fail(c, AE_ERR_DEVICE, "device error %d (%s)", h, (h >= 0 && h <= 6) ? names[h] : "?");
 }
 
 // The error word read back on the stream (enqueue before the synchronisation, check after it):
@@ -1151,6 +1160,8 @@ int ae_ctx_destroy(ae_ctx* c) {
   if (c->h_err) cudaFreeHost(c->h_err);
   if (c->d_cu_single) cudaFree(c->d_cu_single);
   if (c->d_gemm_scratch) cudaFree(c->d_gemm_scratch);
+  for (auto& s : c->scratch)
+    if (s.second.p) cudaFree(s.second.p);
   if (c->own_stream) cudaStreamDestroy(c->own_stream);
   delete c;
   return 0;
@@ -1671,6 +1682,191 @@ int ae_attention_i8(ae_ctx* c, const float* d_qkv, const uint32_t* d_cu, uint32_
   a.err = c->d_err;
   ++c->launches;
   if (launch_attention_i8(a, int(n), 1, c->stream)) return fail(c, AE_ERR_CUDA, "int8 attention launch failed");
+  return 0;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Scratch of at least `bytes` for the context's present stream (grown by half again, never shrunk).
+int stream_scratch(ae_ctx* c, size_t bytes, uint8_t** out) {
+  try {
+    auto& s = c->scratch[c->stream];
+    if (s.bytes < bytes) {
+      if (s.p) {
+        CUDA_TRY(c, cudaStreamSynchronize(c->stream));
+        cudaFree(s.p);
+        s.p = nullptr;
+      }
+      const size_t want = std::max(bytes, s.bytes + s.bytes / 2);
+      s.bytes = 0;
+      CUDA_TRY(c, cudaMalloc(&s.p, want));
+      s.bytes = want;
+    }
+    *out = s.p;
+    return 0;
+  } catch (const std::bad_alloc&) {
+    return fail(c, AE_ERR_CUDA, "out of host memory");
+  }
+}
+
+bool float_type(int t) { return t == AE_F32 || t == AE_F16 || t == AE_BF16; }
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+constexpr uint32_t kMaxProductRows = 1u << 30;
+constexpr uint32_t kMaxProductDepth = 131071;  // 128 * 128 * depth stays inside int32
+
+// The checks ae_matmul_i8 and ae_linear_i8 share, and their arguments as the kernels take them.
+int product_args(ae_ctx* c, const char* who, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_w, uint64_t ldw,
+                 const float* d_w_scale, const float* d_bias, int out_type, void* d_out, uint64_t ldo,
+                 ProductArgs* out) {
+  if (!float_type(out_type)) return fail(c, AE_ERR_INVALID_ARG, "%s: unknown output type %d", who, out_type);
+  if (M > kMaxProductRows || N == 0 || N > kMaxProductRows || K == 0 || K > kMaxProductDepth)
+    return fail(c, AE_ERR_INVALID_ARG, "%s: M 0..2^30, N 1..2^30, K 1..131071 (got %u, %u, %u)", who, M, N, K);
+  if (!d_w || !d_w_scale || (M && !d_out)) return fail(c, AE_ERR_INVALID_ARG, "%s: null operand", who);
+  if (ldw < K || ldo < N) return fail(c, AE_ERR_INVALID_ARG, "%s: row pitch below the row length", who);
+  if (ldw >> 39 || ldo >> 39) return fail(c, AE_ERR_INVALID_ARG, "%s: row pitch over 2^39", who);
+  if (!aligned(d_w_scale, 4) || !aligned(d_bias, 4) || !aligned(d_out, float_type_bytes(out_type)))
+    return fail(c, AE_ERR_INVALID_ARG, "%s: pointer not aligned to its element", who);
+  ProductArgs a{};
+  a.M = int(M);
+  a.N = int(N);
+  a.K = int(K);
+  a.w = d_w;
+  a.ldw = ldw;
+  a.w_scale = d_w_scale;
+  a.bias = d_bias;
+  a.out = d_out;
+  a.ldo = ldo;
+  a.out_type = out_type;
+  a.err = c->d_err;
+  *out = a;
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ae_matmul_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_a, uint64_t lda,
+                 const float* d_a_scale, const int8_t* d_w, uint64_t ldw, const float* d_w_scale, const float* d_bias,
+                 int out_type, void* d_out, uint64_t ldo) {
+  if (!c) return AE_ERR_INVALID_ARG;
+  ProductArgs a;
+  AE_TRY(product_args(c, "ae_matmul_i8", M, N, K, d_w, ldw, d_w_scale, d_bias, out_type, d_out, ldo, &a));
+  if (M && (!d_a || !d_a_scale)) return fail(c, AE_ERR_INVALID_ARG, "ae_matmul_i8: null operand");
+  if (lda < K || lda >> 39) return fail(c, AE_ERR_INVALID_ARG, "ae_matmul_i8: bad row pitch");
+  if (!aligned(d_a_scale, 4)) return fail(c, AE_ERR_INVALID_ARG, "ae_matmul_i8: pointer not aligned to its element");
+  if (M == 0) return 0;
+  DeviceGuard g(c->device);
+  a.a = d_a;
+  a.lda = lda;
+  a.a_scale = d_a_scale;
+  ++c->launches;
+  if (launch_product_i8(a, c->stream)) return fail(c, AE_ERR_CUDA, "int8 product launch failed");
+  return 0;
+}
+
+int ae_linear_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, int x_type, const void* d_x, uint64_t ldx,
+                 const float* d_inv_smooth, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
+                 const float* d_bias, int out_type, void* d_out, uint64_t ldo) {
+  if (!c) return AE_ERR_INVALID_ARG;
+  ProductArgs a;
+  AE_TRY(product_args(c, "ae_linear_i8", M, N, K, d_w, ldw, d_w_scale, d_bias, out_type, d_out, ldo, &a));
+  if (!float_type(x_type)) return fail(c, AE_ERR_INVALID_ARG, "ae_linear_i8: unknown input type %d", x_type);
+  if (M && !d_x) return fail(c, AE_ERR_INVALID_ARG, "ae_linear_i8: null operand");
+  if (ldx < K || ldx >> 39) return fail(c, AE_ERR_INVALID_ARG, "ae_linear_i8: bad row pitch");
+  if (!aligned(d_x, float_type_bytes(x_type)) || !aligned(d_inv_smooth, 4))
+    return fail(c, AE_ERR_INVALID_ARG, "ae_linear_i8: pointer not aligned to its element");
+  if (M == 0) return 0;
+  DeviceGuard g(c->device);
+  QuantArgs q{};
+  q.M = int(M);
+  q.K = int(K);
+  q.x = d_x;
+  q.ldx = ldx;
+  q.x_type = x_type;
+  q.inv_smooth = d_inv_smooth;
+  q.ldq = align_up(K, 16);
+  uint8_t* scratch = nullptr;
+  const size_t q_bytes = align_up(q.ldq * M, 256);
+  AE_TRY(stream_scratch(c, q_bytes + size_t(M) * sizeof(float), &scratch));
+  q.q = reinterpret_cast<int8_t*>(scratch);
+  q.scale = reinterpret_cast<float*>(scratch + q_bytes);
+  c->launches += 2;
+  if (launch_quant_rows(q, c->stream)) return fail(c, AE_ERR_CUDA, "row quantization launch failed");
+  a.a = q.q;
+  a.lda = q.ldq;
+  a.a_scale = q.scale;
+  if (launch_product_i8(a, c->stream)) return fail(c, AE_ERR_CUDA, "int8 product launch failed");
+  return 0;
+}
+
+int ae_qk_norm_rope(ae_ctx* c, int type, uint32_t tokens, uint32_t q_heads, uint32_t k_heads, uint32_t head_dim,
+                    uint32_t rotary_dim, int flags, const void* d_q, uint64_t q_token_stride, uint64_t q_head_stride,
+                    const void* d_k, uint64_t k_token_stride, uint64_t k_head_stride, void* d_q_out,
+                    uint64_t q_out_token_stride, uint64_t q_out_head_stride, void* d_k_out,
+                    uint64_t k_out_token_stride, uint64_t k_out_head_stride, const float* d_q_weight,
+                    const float* d_k_weight, float eps, const float* d_table, uint32_t table_rows,
+                    const int32_t* d_positions, const uint32_t* d_cu_seqlens, uint32_t n_seqs) {
+  if (!c) return AE_ERR_INVALID_ARG;
+  const char* who = "ae_qk_norm_rope";
+  if (!float_type(type)) return fail(c, AE_ERR_INVALID_ARG, "%s: unknown type %d", who, type);
+  if (flags & ~(AE_QK_NEIGHBOURS | AE_QK_NO_NORM)) return fail(c, AE_ERR_INVALID_ARG, "%s: unknown flags %d", who, flags);
+  if (head_dim == 0 || head_dim > 512 || rotary_dim > head_dim || rotary_dim % 2)
+    return fail(c, AE_ERR_INVALID_ARG, "%s: head_dim 1..512 and an even rotary_dim up to it (got %u, %u)", who, head_dim,
+                rotary_dim);
+  if (q_heads > 65535 || k_heads > 65535 || tokens > 1u << 30)
+    return fail(c, AE_ERR_INVALID_ARG, "%s: at most 65,535 heads of a kind and 2^30 tokens", who);
+  if (!(eps >= 0.0f)) return fail(c, AE_ERR_INVALID_ARG, "%s: eps must not be negative", who);
+  if (tokens == 0 || q_heads + k_heads == 0) return 0;
+  if ((q_heads && (!d_q || !d_q_out)) || (k_heads && (!d_k || !d_k_out)))
+    return fail(c, AE_ERR_INVALID_ARG, "%s: null heads", who);
+  if (rotary_dim && (!d_table || table_rows == 0 || table_rows > 1u << 30))
+    return fail(c, AE_ERR_INVALID_ARG, "%s: a rotation needs a table of 1..2^30 rows", who);
+  if (rotary_dim && !d_positions && (!d_cu_seqlens || n_seqs == 0 || n_seqs > 1u << 30))
+    return fail(c, AE_ERR_INVALID_ARG, "%s: a rotation needs positions, or cu_seqlens of 1..2^30 sequences", who);
+  const size_t e = float_type_bytes(type);
+  if (!aligned(d_q, e) || !aligned(d_k, e) || !aligned(d_q_out, e) || !aligned(d_k_out, e) || !aligned(d_q_weight, 4) ||
+      !aligned(d_k_weight, 4) || !aligned(d_table, 4) || !aligned(d_positions, 4) || !aligned(d_cu_seqlens, 4))
+    return fail(c, AE_ERR_INVALID_ARG, "%s: pointer not aligned to its element", who);
+  for (uint64_t s : {q_token_stride, q_head_stride, k_token_stride, k_head_stride, q_out_token_stride,
+                     q_out_head_stride, k_out_token_stride, k_out_head_stride})
+    if (s >> 32) return fail(c, AE_ERR_INVALID_ARG, "%s: stride over 2^32 elements", who);
+  DeviceGuard g(c->device);
+  QkArgs a{};
+  a.tokens = int(tokens);
+  a.heads[0] = int(q_heads);
+  a.heads[1] = int(k_heads);
+  a.dim = int(head_dim);
+  a.rotary = int(rotary_dim);
+  a.type = type;
+  a.neighbours = (flags & AE_QK_NEIGHBOURS) != 0;
+  a.norm = (flags & AE_QK_NO_NORM) == 0;
+  a.x[0] = d_q;
+  a.x[1] = d_k;
+  a.x_ts[0] = q_token_stride;
+  a.x_ts[1] = k_token_stride;
+  a.x_hs[0] = q_head_stride;
+  a.x_hs[1] = k_head_stride;
+  a.y[0] = d_q_out;
+  a.y[1] = d_k_out;
+  a.y_ts[0] = q_out_token_stride;
+  a.y_ts[1] = k_out_token_stride;
+  a.y_hs[0] = q_out_head_stride;
+  a.y_hs[1] = k_out_head_stride;
+  a.weight[0] = a.norm ? d_q_weight : nullptr;
+  a.weight[1] = a.norm ? d_k_weight : nullptr;
+  a.eps = eps;
+  a.table = d_table;
+  a.table_rows = int(table_rows);
+  a.positions = d_positions;
+  a.cu = d_cu_seqlens;
+  a.n_seqs = int(n_seqs);
+  a.err = c->d_err;
+  ++c->launches;
+  if (launch_qk_norm_rope(a, c->stream)) return fail(c, AE_ERR_CUDA, "norm and rotation launch failed");
   return 0;
 }
 

@@ -1,0 +1,185 @@
+// General int8 product with a scale for each token and each output channel, and the per-token
+// quantization that feeds it from float activations:
+//
+//   y = x * inv_smooth;  top = max_k |y|;  a = round_half_even(y * (127 / top));  a_scale = top / 127
+//   out[m, n] = fma(float(sum_k a[m, k] w[n, k]), a_scale[m] * w_scale[n], bias[n])
+//
+// The integer sum is exact, so the only roundings are float(sum), the product of the scales, the fused
+// multiply-add, and one to the output's type.
+#include "linear_i8.h"
+
+#include "floatio.cuh"
+#include "ptx.cuh"
+#include "rowmath.cuh"
+
+namespace ae {
+
+// Smallest row maximum that quantizes to anything but zeros: below it 127 / top would not be finite.
+constexpr float kTinyTop = 0x1p-119f;
+
+// ------------------------------------------------------------------------------- row quantization
+// TPR threads to a row. The row is read once into registers (NV 16-byte pieces a thread), or, when it is
+// longer than that (NV = 0), twice, the second time from L2.
+template <class T, int TPR, int NV>
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) k_quant_rows(QuantArgs a) {
+  constexpr int VE = kPiece<T>;
+  constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
+  pdl_trigger();
+  pdl_wait();
+  const int row = blockIdx.x * RPB + threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const bool live = row < a.M;
+  const T* x = static_cast<const T*>(a.x) + (live ? size_t(row) * a.ldx : 0);
+  const bool wide = ((reinterpret_cast<uintptr_t>(a.x) | (a.ldx * sizeof(T))) & 15) == 0;
+  const int pieces = (a.K + VE - 1) / VE;
+
+  auto load = [&](int p, float (&v)[VE]) {
+    const int k = p * VE;
+    if (wide && k + VE <= a.K) {
+      widen<T>(*reinterpret_cast<const uint4*>(x + k), v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = k + e < a.K ? to_f32(x[k + e]) : 0.0f;
+    }
+    if (a.inv_smooth) {
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        if (k + e < a.K) v[e] *= a.inv_smooth[k + e];
+    }
+  };
+  // |y| compared by its bits: the order is the same, and a NaN is above every number
+  uint32_t top = 0;
+  auto take = [&](const float (&v)[VE]) {
+#pragma unroll
+    for (int e = 0; e < VE; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+  };
+  float keep[NV > 0 ? NV : 1][VE];
+  if (live) {
+    if constexpr (NV > 0) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (t + i * TPR < pieces) {
+          load(t + i * TPR, keep[i]);
+          take(keep[i]);
+        }
+    } else {
+      for (int p = t; p < pieces; p += TPR) {
+        load(p, keep[0]);
+        take(keep[0]);
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (TPR > 32) {
+    __shared__ uint32_t s_top[TPR / 32];
+    if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TPR / 32; ++w) top = max(top, s_top[w]);
+  }
+  if (!live) return;
+  // a row that holds an infinity or a NaN has no scale: its scale is NaN, and so is its row of the product
+  const bool finite = top < 0x7f800000u;
+  const float m = __uint_as_float(top);
+  const bool any = finite && m >= kTinyTop;
+  const float inv = any ? 127.0f / m : 0.0f;
+  if (t == 0) a.scale[row] = finite ? (any ? m / 127.0f : 0.0f) : __uint_as_float(0x7fc00000u);
+  int8_t* q = a.q + size_t(row) * a.ldq;
+  auto store = [&](int p, const float (&v)[VE]) {
+    uint32_t w[VE / 4];
+#pragma unroll
+    for (int j = 0; j < VE / 4; ++j)
+      w[j] = !any ? 0u
+                  : pack_i8x4(quant_bits_scaled(v[4 * j] * inv), quant_bits_scaled(v[4 * j + 1] * inv),
+                              quant_bits_scaled(v[4 * j + 2] * inv), quant_bits_scaled(v[4 * j + 3] * inv));
+    if constexpr (VE == 8)
+      *reinterpret_cast<uint2*>(q + p * VE) = make_uint2(w[0], w[1]);
+    else
+      *reinterpret_cast<uint32_t*>(q + p * VE) = w[0];
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (t + i * TPR < pieces) store(t + i * TPR, keep[i]);
+  } else {
+    for (int p = t; p < pieces; p += TPR) {
+      load(p, keep[0]);
+      store(p, keep[0]);
+    }
+  }
+}
+
+template <class T, int TPR, int NV>
+static cudaError_t quant(const QuantArgs& a, cudaStream_t st) {
+  constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
+  k_quant_rows<T, TPR, NV><<<(a.M + RPB - 1) / RPB, TPR < 128 ? 128 : TPR, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+// A warp holds 4 pieces a thread (1,024 16-bit values), 128 threads 4,096, 512 threads 16,384.
+template <class T>
+static cudaError_t quant_type(const QuantArgs& a, cudaStream_t st) {
+  const int pieces = (a.K + kPiece<T> - 1) / kPiece<T>;
+  if (pieces <= 32 * 4) return quant<T, 32, 4>(a, st);
+  if (pieces <= 128 * 4) return quant<T, 128, 4>(a, st);
+  if (pieces <= 512 * 4) return quant<T, 512, 4>(a, st);
+  return quant<T, 512, 0>(a, st);
+}
+
+int launch_quant_rows(const QuantArgs& a, cudaStream_t st) {
+  const cudaError_t e = a.x_type == FT_F32   ? quant_type<float>(a, st)
+                        : a.x_type == FT_F16 ? quant_type<__half>(a, st)
+                                             : quant_type<__nv_bfloat16>(a, st);
+  return e == cudaSuccess ? 0 : -100 - int(e);
+}
+
+// ---------------------------------------------------------------------------------------- product
+// 64 tokens x 64 channels to a block, 4 x 4 to a thread, the depth in steps of 64 bytes.
+template <class T>
+__global__ void __launch_bounds__(256) k_product_i8(ProductArgs a) {
+  __shared__ uint32_t sa[64][17], sw[64][17];
+  uint8_t* ba = reinterpret_cast<uint8_t*>(sa);
+  uint8_t* bw = reinterpret_cast<uint8_t*>(sw);
+  const int tiles_n = (a.N + 63) / 64;
+  const int n0 = int(blockIdx.x % tiles_n) * 64, m0 = int(blockIdx.x / tiles_n) * 64;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  int acc[4][4] = {};
+  for (int k0 = 0; k0 < a.K; k0 += 64) {
+    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
+      const int r = i / 64, c = i % 64, k = k0 + c;
+      ba[r * 68 + c] = (m0 + r < a.M && k < a.K) ? uint8_t(a.a[size_t(m0 + r) * a.lda + k]) : 0;
+      bw[r * 68 + c] = (n0 + r < a.N && k < a.K) ? uint8_t(a.w[size_t(n0 + r) * a.ldw + k]) : 0;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int c = 0; c < 16; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(int(sa[ty + 16 * i][c]), int(sw[tx + 16 * j][c]), acc[i][j]);
+    __syncthreads();
+  }
+  for (int i = 0; i < 4; ++i) {
+    const int m = m0 + ty + 16 * i;
+    if (m >= a.M) continue;
+    const float as = a.a_scale[m];
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + tx + 16 * j;
+      if (n < a.N)
+        static_cast<T*>(a.out)[size_t(m) * a.ldo + n] =
+            from_f32<T>(fmaf(float(acc[i][j]), as * a.w_scale[n], a.bias ? a.bias[n] : 0.0f));
+    }
+  }
+}
+
+int launch_product_i8(const ProductArgs& a, cudaStream_t st) {
+  const long long blocks = (long long)((a.M + 63) / 64) * ((a.N + 63) / 64);
+  if (blocks > 0x7fffffffll) return -1;
+  if (a.out_type == FT_F32) k_product_i8<float><<<unsigned(blocks), 256, 0, st>>>(a);
+  else if (a.out_type == FT_F16) k_product_i8<__half><<<unsigned(blocks), 256, 0, st>>>(a);
+  else k_product_i8<__nv_bfloat16><<<unsigned(blocks), 256, 0, st>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : -100 - int(e);
+}
+
+}  // namespace ae

@@ -18,6 +18,7 @@ enum DevErr : int {
   DEV_ERR_TIMEOUT_EPILOGUE = 3,
   DEV_ERR_BAD_SHAPE = 4,
   DEV_ERR_BAD_TOKEN = 5,
+  DEV_ERR_BAD_POSITION = 6,
 };
 
 // Wait limit: 2 s of wall time, far above any legitimate wait inside one launch.

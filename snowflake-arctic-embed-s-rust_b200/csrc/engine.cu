@@ -1745,6 +1745,17 @@ int product_args(ae_ctx* c, const char* who, uint32_t M, uint32_t N, uint32_t K,
   return 0;
 }
 
+// The product; scratch: what product_scratch asks for, or nullptr to take it from the stream's here.
+int product(ae_ctx* c, const ProductArgs& a, uint8_t* scratch, int tokens_ahead) {
+  const size_t need = product_scratch(a);
+  if (need && !scratch) AE_TRY(stream_scratch(c, need, &scratch));
+  int kernels = 0;
+  const int r = launch_product_i8(a, scratch, tokens_ahead, c->stream, &kernels);
+  c->launches += kernels;
+  if (r) return fail(c, AE_ERR_CUDA, "int8 product launch failed: code %d", r);
+  return 0;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1763,9 +1774,7 @@ int ae_matmul_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_
   a.a = d_a;
   a.lda = lda;
   a.a_scale = d_a_scale;
-  ++c->launches;
-  if (launch_product_i8(a, c->stream)) return fail(c, AE_ERR_CUDA, "int8 product launch failed");
-  return 0;
+  return product(c, a, nullptr, 0);
 }
 
 int ae_linear_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, int x_type, const void* d_x, uint64_t ldx,
@@ -1790,17 +1799,16 @@ int ae_linear_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, int x_type, cons
   q.inv_smooth = d_inv_smooth;
   q.ldq = align_up(K, 16);
   uint8_t* scratch = nullptr;
-  const size_t q_bytes = align_up(q.ldq * M, 256);
-  AE_TRY(stream_scratch(c, q_bytes + size_t(M) * sizeof(float), &scratch));
+  const size_t q_bytes = align_up(q.ldq * M, 256), s_bytes = align_up(size_t(M) * sizeof(float), 256);
+  a.lda = q.ldq;
+  AE_TRY(stream_scratch(c, q_bytes + s_bytes + product_scratch(a), &scratch));
   q.q = reinterpret_cast<int8_t*>(scratch);
   q.scale = reinterpret_cast<float*>(scratch + q_bytes);
-  c->launches += 2;
+  ++c->launches;
   if (launch_quant_rows(q, c->stream)) return fail(c, AE_ERR_CUDA, "row quantization launch failed");
   a.a = q.q;
-  a.lda = q.ldq;
   a.a_scale = q.scale;
-  if (launch_product_i8(a, c->stream)) return fail(c, AE_ERR_CUDA, "int8 product launch failed");
-  return 0;
+  return product(c, a, scratch + q_bytes + s_bytes, 1);
 }
 
 int ae_qk_norm_rope(ae_ctx* c, int type, uint32_t tokens, uint32_t q_heads, uint32_t k_heads, uint32_t head_dim,

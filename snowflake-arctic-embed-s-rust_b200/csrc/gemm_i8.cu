@@ -786,12 +786,12 @@ static PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
 }
 
 // Tensor map of a [rows, K] row-major int8 matrix: boxes of box_rows x 128 bytes, 128-byte swizzle.
-int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
+int make_tmap_i8_rows(CUtensorMap* map, const void* base, size_t rows, size_t K, size_t pitch, int box_rows) {
   auto enc = get_encode();
   if (!enc) return -1;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || (K % 16) || rows <= 0) return -2;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (pitch % 16) || rows == 0) return -2;
   cuuint64_t dims[2] = {cuuint64_t(K), cuuint64_t(rows)};
-  cuuint64_t strides[1] = {cuuint64_t(K)};
+  cuuint64_t strides[1] = {cuuint64_t(pitch)};
   cuuint32_t box[2] = {128, cuuint32_t(box_rows)};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
@@ -800,7 +800,12 @@ int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_ro
   return r == CUDA_SUCCESS ? 0 : -3;
 }
 
-static int num_sms() {
+int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_rows) {
+  if (K % 16 || rows <= 0) return -2;
+  return make_tmap_i8_rows(map, base, size_t(rows), size_t(K), size_t(K), box_rows);
+}
+
+int num_sms() {
   static int cache[kMaxDevices] = {};
   int dev = 0;
   cudaGetDevice(&dev);

@@ -38,6 +38,9 @@ int gemm_i8_prime();
 // Tensor map of a [rows, K] row-major int8 matrix with boxes of box_rows x 128 bytes: 128 for
 // activations (A operands), 64 for weights (B operands, loaded in 64-row slices).
 int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_rows);
+// The same for rows `pitch` bytes apart (a multiple of 16); K may be any, bytes past it read as zero.
+int make_tmap_i8_rows(CUtensorMap* map, const void* base, size_t rows, size_t K, size_t pitch, int box_rows);
+int num_sms();  // of the current device
 constexpr int kBoxA = 128;
 constexpr int kBoxB = 64;
 int gemm_i8_launch(int epi, const CUtensorMap& ta, const CUtensorMap& tb, const GemmArgs& g, cudaStream_t st);

@@ -1,14 +1,10 @@
-// General int8 product with a scale for each token and each output channel, and the per-token
-// quantization that feeds it from float activations:
+// Per-token quantization of float activations, the int8 operand of the general product (product_i8.cu):
 //
 //   y = x * inv_smooth;  top = max_k |y|;  a = round_half_even(y * (127 / top));  a_scale = top / 127
-//   out[m, n] = fma(float(sum_k a[m, k] w[n, k]), a_scale[m] * w_scale[n], bias[n])
-//
-// The integer sum is exact, so the only roundings are float(sum), the product of the scales, the fused
-// multiply-add, and one to the output's type.
 #include "linear_i8.h"
 
 #include "floatio.cuh"
+#include "kernels.h"
 #include "ptx.cuh"
 #include "rowmath.cuh"
 
@@ -24,8 +20,9 @@ template <class T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) k_quant_rows(QuantArgs a) {
   constexpr int VE = kPiece<T>;
   constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
-  pdl_trigger();
+  // in this order, so that what starts early behind this kernel finds all work ahead of it done
   pdl_wait();
+  pdl_trigger();
   const int row = blockIdx.x * RPB + threadIdx.x / TPR;
   const int t = threadIdx.x % TPR;
   const bool live = row < a.M;
@@ -112,8 +109,7 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) k_quant_rows(QuantArgs 
 template <class T, int TPR, int NV>
 static cudaError_t quant(const QuantArgs& a, cudaStream_t st) {
   constexpr int RPB = TPR < 128 ? 128 / TPR : 1;
-  k_quant_rows<T, TPR, NV><<<(a.M + RPB - 1) / RPB, TPR < 128 ? 128 : TPR, 0, st>>>(a);
-  return cudaGetLastError();
+  return launch_pdl(k_quant_rows<T, TPR, NV>, dim3((a.M + RPB - 1) / RPB), dim3(TPR < 128 ? 128 : TPR), 0, st, a);
 }
 
 // A warp holds 4 pieces a thread (1,024 16-bit values), 128 threads 4,096, 512 threads 16,384.
@@ -130,55 +126,6 @@ int launch_quant_rows(const QuantArgs& a, cudaStream_t st) {
   const cudaError_t e = a.x_type == FT_F32   ? quant_type<float>(a, st)
                         : a.x_type == FT_F16 ? quant_type<__half>(a, st)
                                              : quant_type<__nv_bfloat16>(a, st);
-  return e == cudaSuccess ? 0 : -100 - int(e);
-}
-
-// ---------------------------------------------------------------------------------------- product
-// 64 tokens x 64 channels to a block, 4 x 4 to a thread, the depth in steps of 64 bytes.
-template <class T>
-__global__ void __launch_bounds__(256) k_product_i8(ProductArgs a) {
-  __shared__ uint32_t sa[64][17], sw[64][17];
-  uint8_t* ba = reinterpret_cast<uint8_t*>(sa);
-  uint8_t* bw = reinterpret_cast<uint8_t*>(sw);
-  const int tiles_n = (a.N + 63) / 64;
-  const int n0 = int(blockIdx.x % tiles_n) * 64, m0 = int(blockIdx.x / tiles_n) * 64;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  int acc[4][4] = {};
-  for (int k0 = 0; k0 < a.K; k0 += 64) {
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-      const int r = i / 64, c = i % 64, k = k0 + c;
-      ba[r * 68 + c] = (m0 + r < a.M && k < a.K) ? uint8_t(a.a[size_t(m0 + r) * a.lda + k]) : 0;
-      bw[r * 68 + c] = (n0 + r < a.N && k < a.K) ? uint8_t(a.w[size_t(n0 + r) * a.ldw + k]) : 0;
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int c = 0; c < 16; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(int(sa[ty + 16 * i][c]), int(sw[tx + 16 * j][c]), acc[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; ++i) {
-    const int m = m0 + ty + 16 * i;
-    if (m >= a.M) continue;
-    const float as = a.a_scale[m];
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + tx + 16 * j;
-      if (n < a.N)
-        static_cast<T*>(a.out)[size_t(m) * a.ldo + n] =
-            from_f32<T>(fmaf(float(acc[i][j]), as * a.w_scale[n], a.bias ? a.bias[n] : 0.0f));
-    }
-  }
-}
-
-int launch_product_i8(const ProductArgs& a, cudaStream_t st) {
-  const long long blocks = (long long)((a.M + 63) / 64) * ((a.N + 63) / 64);
-  if (blocks > 0x7fffffffll) return -1;
-  if (a.out_type == FT_F32) k_product_i8<float><<<unsigned(blocks), 256, 0, st>>>(a);
-  else if (a.out_type == FT_F16) k_product_i8<__half><<<unsigned(blocks), 256, 0, st>>>(a);
-  else k_product_i8<__nv_bfloat16><<<unsigned(blocks), 256, 0, st>>>(a);
-  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -100 - int(e);
 }
 

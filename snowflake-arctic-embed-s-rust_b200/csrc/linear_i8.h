@@ -40,7 +40,11 @@ struct QuantArgs {
 };
 
 int launch_quant_rows(const QuantArgs& a, cudaStream_t st);
-int launch_product_i8(const ProductArgs& a, cudaStream_t st);
+// Scratch (256-byte aligned) for the operands whose rows TMA cannot read where they are.
+size_t product_scratch(const ProductArgs& a);
+// tokens_ahead: the kernel launched right before on st is this call's launch_quant_rows, so all work ahead of
+// that one (whatever wrote the weights) is done once the product starts. *kernels += the launches made.
+int launch_product_i8(const ProductArgs& a, uint8_t* scratch, int tokens_ahead, cudaStream_t st, int* kernels);
 
 struct QkArgs {
   int tokens, heads[2], dim, rotary;  // heads[0] queries, heads[1] keys

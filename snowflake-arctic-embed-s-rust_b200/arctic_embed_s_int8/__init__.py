@@ -53,33 +53,69 @@ def _ptr(a) -> int | None:
     return a.data_ptr()  # torch tensor (device memory)
 
 
-# element types of the general operators' float tensors (AE_F32 / AE_F16 / AE_BF16)
-_FLOAT_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+class _TensorTypes:
+    """torch's dtypes as the general operators take them, looked up once: a call's checks cost about as much as
+    its launch on small inputs."""
+
+    def __init__(self):
+        import torch
+
+        self.i8, self.i32, self.f32 = torch.int8, torch.int32, torch.float32
+        self.offsets = (torch.int32, torch.uint32)
+        self.floats = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # AE_F32 / AE_F16 / AE_BF16
 
 
-def _float_type(t, what: str) -> int:
-    code = _FLOAT_TYPES.get(str(t.dtype))
-    if code is None:
-        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
-    return code
+_tensor_types = None
 
 
-def _operand(t, what: str, shape: tuple, dtype: str, device: int):
-    """A tensor of this shape and type in device memory of GPU `device`, its last axis contiguous."""
-    if tuple(t.shape) != shape:
+def _types() -> _TensorTypes:
+    global _tensor_types
+    if _tensor_types is None:
+        _tensor_types = _TensorTypes()
+    return _tensor_types
+
+
+def _refuse(t, what: str, shape: tuple, dtype, device: int):
+    if t.shape != shape:
         raise ValueError(f"{what} must be {shape}, not {tuple(t.shape)}")
-    if dtype is not None and str(t.dtype) != dtype:
+    if t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
-    if not t.is_cuda or t.get_device() != device:
+    if t.get_device() != device:
         raise ValueError(f"{what} must be in device memory of GPU {device}")
-    if t.stride(-1) != 1 and shape[-1] > 1 and t.numel():
-        raise ValueError(f"{what} must be contiguous along its last axis")
+    raise ValueError(f"{what} must be contiguous along its last axis")
+
+
+def _vector(t, what: str, n: int, dtype, device: int) -> int:
+    """Address of a contiguous [n] device tensor."""
+    if t.shape != (n,) or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        _refuse(t, what, (n,), dtype, device)
     return t.data_ptr()
 
 
-def _pitch(t) -> int:
-    """Row pitch of a 2-D tensor in elements; that of a single row is the row's own length."""
-    return t.stride(0) if t.shape[0] > 1 and t.shape[1] else t.shape[1]
+def _matrix(t, what: str, rows: int, cols: int, dtype, device: int) -> tuple[int, int]:
+    """Address and row pitch of a [rows, cols] device tensor whose rows are contiguous; the pitch of a single
+    row is the row's own length."""
+    pitch, step = t.stride()
+    if t.shape != (rows, cols) or t.dtype is not dtype or t.get_device() != device or (
+            step != 1 and cols > 1 and rows):
+        _refuse(t, what, (rows, cols), dtype, device)
+    return t.data_ptr(), pitch if rows > 1 and cols else cols
+
+
+def _heads(t, what: str, shape: tuple, dtype, device: int) -> tuple[int, int, int]:
+    """Address, token stride and head stride of a [tokens, heads, dim] device tensor with contiguous heads."""
+    token, head, step = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
+            step != 1 and shape[2] > 1 and t.numel()):
+        _refuse(t, what, shape, dtype, device)
+    return t.data_ptr(), token, head
+
+
+def _float_type(t, what: str) -> int:
+    code = _types().floats.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
 
 
 def _linear_desc(lin: ae8.QuantizedLinear | None, keep: list) -> LinearDesc:
@@ -222,37 +258,37 @@ class Engine:
         """ae_attention_i8: the reference's int8 attention scheme on device buffers (every sequence)."""
         self._check(lib().ae_attention_i8(self._h, _ptr(qkv), _ptr(cu), n_seqs, max_len, _ptr(ctx)))
 
-    def _weights(self, w, w_scale, bias, out, M: int):
-        """The checks and arguments matmul_i8 and linear_i8 share."""
-        if w.dim() != 2:
-            raise ValueError("w must be [out_features, in_features]")
-        N, K = w.shape
-        dev = self.device
-        return (N, K, (_operand(w, "w", (N, K), "torch.int8", dev), _pitch(w),
-                       _operand(w_scale, "w_scale", (N,), "torch.float32", dev),
-                       None if bias is None else _operand(bias, "bias", (N,), "torch.float32", dev)),
-                (_float_type(out, "out"), _operand(out, "out", (M, N), None, dev), _pitch(out)))
-
     def matmul_i8(self, a, a_scale, w, w_scale, out, bias=None) -> None:
         """ae_matmul_i8: out[m, n] = (sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n]) + bias[n] on device
         tensors: a [M, K] and w [N, K] int8, a_scale [M], w_scale [N] and bias [N] float32, out [M, N]
         float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream."""
-        M = a.shape[0]
-        N, K, weights, result = self._weights(w, w_scale, bias, out, M)
-        self._check(lib().ae_matmul_i8(self._h, M, N, K, _operand(a, "a", (M, K), "torch.int8", self.device),
-                                       _pitch(a),
-                                       _operand(a_scale, "a_scale", (M,), "torch.float32", self.device), *weights,
-                                       *result))
+        ty, dev = _types(), self.device
+        (M, K), N = a.shape, w.shape[0]
+        out_type = _float_type(out, "out")
+        ap, lda = _matrix(a, "a", M, K, ty.i8, dev)
+        wp, ldw = _matrix(w, "w", N, K, ty.i8, dev)
+        op, ldo = _matrix(out, "out", M, N, out.dtype, dev)
+        code = lib().ae_matmul_i8(self._h, M, N, K, ap, lda, _vector(a_scale, "a_scale", M, ty.f32, dev), wp, ldw,
+                                  _vector(w_scale, "w_scale", N, ty.f32, dev),
+                                  None if bias is None else _vector(bias, "bias", N, ty.f32, dev), out_type, op, ldo)
+        if code:
+            self._check(code)
 
     def linear_i8(self, x, w, w_scale, out, bias=None, inv_smooth=None) -> None:
         """ae_linear_i8: the same product from float activations x [M, K] (float32, float16 or bfloat16),
         multiplied by inv_smooth [K] and quantized to int8 with a scale for each token on the way."""
-        M = x.shape[0]
-        N, K, weights, result = self._weights(w, w_scale, bias, out, M)
-        dev = self.device
-        smooth = None if inv_smooth is None else _operand(inv_smooth, "inv_smooth", (K,), "torch.float32", dev)
-        self._check(lib().ae_linear_i8(self._h, M, N, K, _float_type(x, "x"), _operand(x, "x", (M, K), None, dev),
-                                       _pitch(x), smooth, *weights, *result))
+        ty, dev = _types(), self.device
+        (M, K), N = x.shape, w.shape[0]
+        x_type, out_type = _float_type(x, "x"), _float_type(out, "out")
+        xp, ldx = _matrix(x, "x", M, K, x.dtype, dev)
+        wp, ldw = _matrix(w, "w", N, K, ty.i8, dev)
+        op, ldo = _matrix(out, "out", M, N, out.dtype, dev)
+        code = lib().ae_linear_i8(self._h, M, N, K, x_type, xp, ldx,
+                                  None if inv_smooth is None else _vector(inv_smooth, "inv_smooth", K, ty.f32, dev),
+                                  wp, ldw, _vector(w_scale, "w_scale", N, ty.f32, dev),
+                                  None if bias is None else _vector(bias, "bias", N, ty.f32, dev), out_type, op, ldo)
+        if code:
+            self._check(code)
 
     QK_NEIGHBOURS, QK_NO_NORM = 1, 2
 
@@ -262,32 +298,37 @@ class Engine:
         k [T, k_heads, dim] and the rotation of their first table.shape[1] dims, into q_out and k_out (which
         may be q and k). table [rows, rotary] float32 is rope_table's; a token's position is positions[t]
         (int32), or its place in its sequence of cu (int32 or uint32 [n_seqs + 1])."""
-        T, Hq, D = q.shape
-        Hk, dev, dt, code = k.shape[1], self.device, str(q.dtype), _float_type(q, "q")
-        heads = ()
-        for t, what, H in ((q, "q", Hq), (k, "k", Hk), (q_out, "q_out", Hq), (k_out, "k_out", Hk)):
-            heads += (_operand(t, what, (T, H, D), dt, dev), t.stride(0), t.stride(1))
+        ty, dev, dt = _types(), self.device, q.dtype
+        code = _float_type(q, "q")
+        T, Hq, D = shape = q.shape
+        Hk = k.shape[1]
+        k_shape = (T, Hk, D)
         rows = rotary = n_seqs = 0
         tp = pp = cp = None
         if table is not None:
             rows, rotary = table.shape
-            if not table.is_contiguous():
+            tp, pitch = _matrix(table, "table", rows, rotary, ty.f32, dev)
+            if pitch != rotary:
                 raise ValueError("table must be contiguous")
-            tp = _operand(table, "table", (rows, rotary), "torch.float32", dev)
             if positions is not None:
-                pp = _operand(positions, "positions", (T,), "torch.int32", dev)
+                pp = _vector(positions, "positions", T, ty.i32, dev)
             elif cu is not None:
-                n_seqs = len(cu) - 1
-                if str(cu.dtype) not in ("torch.int32", "torch.uint32"):
+                n_seqs = cu.shape[0] - 1
+                if cu.dtype not in ty.offsets:
                     raise ValueError(f"cu must be int32 or uint32, not {cu.dtype}")
-                cp = _operand(cu, "cu", (n_seqs + 1,), None, dev)
+                cp = _vector(cu, "cu", n_seqs + 1, cu.dtype, dev)
             else:
                 raise ValueError("a rotation needs positions or cu")
-        qw = None if q_weight is None else _operand(q_weight, "q_weight", (D,), "torch.float32", dev)
-        kw = None if k_weight is None else _operand(k_weight, "k_weight", (D,), "torch.float32", dev)
-        flags = (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM)
-        self._check(lib().ae_qk_norm_rope(self._h, code, T, Hq, Hk, D, rotary, flags, *heads, qw, kw, eps, tp, rows,
-                                          pp, cp, n_seqs))
+        code = lib().ae_qk_norm_rope(
+            self._h, code, T, Hq, Hk, D, rotary,
+            (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM),
+            *_heads(q, "q", shape, dt, dev), *_heads(k, "k", k_shape, dt, dev),
+            *_heads(q_out, "q_out", shape, dt, dev), *_heads(k_out, "k_out", k_shape, dt, dev),
+            None if q_weight is None else _vector(q_weight, "q_weight", D, ty.f32, dev),
+            None if k_weight is None else _vector(k_weight, "k_weight", D, ty.f32, dev),
+            eps, tp, rows, pp, cp, n_seqs)
+        if code:
+            self._check(code)
 
     def set_attention_mode(self, mode: int) -> "Engine":
         """ATTENTION_EXACT (fp32, default) or ATTENTION_INT8 (the reference's int8 scheme) for layers 0-10."""

@@ -422,7 +422,7 @@ Pick pick(int M, int N, int K) {
       best = {bt, mode, split};
     }
   };
-  for (int bt : {16, 32, 64, 128, 256}) {
+  for (int bt = 16; bt <= 256 && (bt == 16 || bt / 2 < M); bt *= 2) {  // none wider than the tokens need
     consider(bt, ONE, 1);
     if (bt >= 128) consider(bt, PAIR, 1);
     if (bt <= 64)

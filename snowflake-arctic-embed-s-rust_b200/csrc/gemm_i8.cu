@@ -805,6 +805,21 @@ int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_ro
   return make_tmap_i8_rows(map, base, size_t(rows), size_t(K), size_t(K), box_rows);
 }
 
+int make_tmap_store(CUtensorMap* map, void* base, size_t rows, size_t cols, size_t pitch, int elem_bytes, int box_rows) {
+  auto enc = get_encode();
+  if (!enc) return -1;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || (pitch % 16) || rows == 0) return -2;
+  cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
+  cuuint64_t strides[1] = {cuuint64_t(pitch)};
+  cuuint32_t box[2] = {32, cuuint32_t(box_rows)};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, elem_bytes == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   elem_bytes == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -3;
+}
+
 int num_sms() {
   static int cache[kMaxDevices] = {};
   int dev = 0;

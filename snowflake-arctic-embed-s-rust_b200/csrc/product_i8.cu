@@ -37,6 +37,7 @@ constexpr int kEpi = 8;                        // epilogue warps
 constexpr int kThreads = 32 * (2 + kEpi);
 constexpr int kSmemMost = 232448;
 constexpr int kMaxSplit = 8;
+constexpr int kBoxBytes = 2048;                // one box of results: 32 channels x 32 (16-bit) or 16 (float) tokens
 constexpr int kGroupM = 8;                     // token tiles walked together, for L2 reuse of the weights
 
 enum Mode { ONE = 0, PAIR = 1, SPLIT = 2 };
@@ -48,7 +49,9 @@ struct Shape {
   static constexpr int T_BYTES = BT / CG * kBlock;
   static constexpr int STAGE = W_BYTES + T_BYTES;
   static constexpr int RED = MODE == SPLIT ? (BT + kMaxSplit) * kChannels * 4 : 0;  // partial sums sent here
-  static constexpr int FIXED = 1024 + RED + 2 * BT * 4 + 512;
+  static constexpr bool BOXES = MODE != SPLIT && BT >= 64;    // results leave as boxes where the output allows
+  static constexpr int OUT = BOXES ? kEpi * 2 * kBoxBytes : 0;
+  static constexpr int FIXED = OUT + RED + 2 * BT * 4 + 256;
   static constexpr int FIT = (kSmemMost - FIXED) / STAGE;
   static constexpr int STAGES = FIT < 12 ? FIT : 12;
   static constexpr int TOTAL = FIXED + STAGES * STAGE;
@@ -60,6 +63,7 @@ struct Grid {
   int tiles_n, tiles_m;
   int split;     // CTAs that share a tile's depth
   int early_w;   // the weights may be read before the kernel ahead has ended
+  int boxes;     // store results as TMA boxes (the output's base and pitch are multiples of 16 bytes)
 };
 
 __device__ __forceinline__ void tile_at(const Grid& g, int tile, int& nt, int& mt) {
@@ -76,21 +80,22 @@ __device__ __forceinline__ void put(T* p, float v) { *p = from_f32<T>(v); }
 
 template <int BT, int MODE, class T>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_product_i8(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_t, ProductArgs a,
-                 Grid g) {
+    k_product_i8(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_t,
+                 const __grid_constant__ CUtensorMap map_o, ProductArgs a, Grid g) {
   using S = Shape<BT, MODE>;
   constexpr int STAGES = S::STAGES;
   constexpr int CG = S::CG;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t* ring = smem;
-  int* red = reinterpret_cast<int*>(ring + STAGES * S::STAGE);
+  extern __shared__ __align__(1024) uint8_t smem_product[];  // the swizzles' 8-row atoms
+  uint8_t* ring = smem_product;
+  uint8_t* s_out = ring + STAGES * S::STAGE;
+  int* red = reinterpret_cast<int*>(s_out + S::OUT);
   float* s_as = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // [2][BT] token scales
   uint64_t* full = reinterpret_cast<uint64_t*>(s_as + 2 * BT);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* red_full = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = MODE == ONE ? 0u : cluster_ctarank();
@@ -112,7 +117,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], kEpi * CG);
     }
+    mbar_init(red_full, 1);
     fence_mbar_init();
+  }
+  // SPLIT: the tile's tokens are finished in runs of `run`, CTA r taking `mine` of them from token r * run on
+  int run = 0, mine = 0;
+  if constexpr (MODE == SPLIT) {
+    int nt, mt;
+    tile_at(g, unit, nt, mt);
+    const int mv = min(BT, a.M - mt * BT);
+    run = (mv + g.split - 1) / g.split;
+    mine = max(0, min(run, mv - int(rank) * run));
+    if (tid == 0 && mine) mbar_arrive_expect_tx(red_full, uint32_t(g.split - 1) * mine * kChannels * 4);
   }
   __syncthreads();
   if constexpr (MODE != ONE) {  // the peers' barriers and shared memory are there before anything reaches for them
@@ -190,6 +206,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      // no load is in flight when the CTA ends, even where the MMAs gave up waiting for one
+      if (MODE != PAIR || rank == 0)
+        for (int i = max(0, kc - STAGES); i < kc; ++i)
+          mbar_wait(&full[i % STAGES], (i / STAGES) & 1, a.err, DEV_ERR_TIMEOUT_PRODUCER);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -234,6 +254,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     bool ok = true;
     int it = 0;
+    [[maybe_unused]] int turn = 0;                  // which of the warp's two boxes
+    [[maybe_unused]] float ws4[4], bias4[4];
     for (int tile = unit; tile < tiles; tile += units, ++it) {
       const int b = it & 1, u = it >> 1;
       int nt, mt;
@@ -252,10 +274,96 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if constexpr (MODE != SPLIT) {
-        constexpr int CW = BT / 2 < 32 ? BT / 2 : 32;  // columns to a TMEM load
-        if (ok) {
+        const int c_end = min(mv, (half + 1) * (BT / 2));
+        auto drained = [&] {  // this warp has read its part of the accumulator
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (MODE == PAIR) mbar_arrive_cluster(map_peer(&acc_empty[b], 0));
+            else mbar_arrive(&acc_empty[b]);
+          }
+        };
+        if (S::BOXES && g.boxes) {
+          if constexpr (S::BOXES) {
+            uint8_t* box0 = s_out + (warp - 2) * 2 * kBoxBytes;
+            const int x = n - lane;
+            constexpr int CT = sizeof(T) == 4 ? 16 : 32;
+            if constexpr (sizeof(T) == 2) {
+              // fragment lanes: channel lane / 4 + 8 i, i = 0..3
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int ni = x + (lane >> 2) + 8 * i;
+                ws4[i] = ni < a.N ? a.w_scale[ni] : 0.0f;
+                bias4[i] = ni < a.N && a.bias ? a.bias[ni] : 0.0f;
+              }
+            }
 #pragma unroll 1
-          for (int c = half * (BT / 2); c < (half + 1) * (BT / 2) && c < mv; c += CW) {
+            for (int c = half * (BT / 2); c < c_end; c += CT, turn ^= 1) {
+              uint8_t* box = box0 + turn * kBoxBytes;
+              const uint32_t at = lane_base + uint32_t(b * BT + c);
+              if (lane == 0) bulk_wait_read<1>();  // the store that left from this box two turns ago
+              if constexpr (sizeof(T) == 2) {
+                uint32_t lo[16], hi[16];
+                if (ok) {
+                  tmem_ld_16x32(at, lo);
+                  tmem_ld_16x32(at + (16u << 16), hi);
+                  tmem_ld_wait();
+                }
+                if (c + CT >= c_end) drained();
+                __syncwarp();
+                const uint32_t row = smem_u32(box) + (lane & 7) * 64;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float2 ts = *reinterpret_cast<const float2*>(as + c + 8 * j + 2 * (lane & 3));
+                  uint32_t p[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const uint32_t* r = (i < 2 ? lo : hi) + 4 * j + 2 * (i & 1);
+                    const float2 v = __ffma2_rn(make_float2(float(int(r[0])), float(int(r[1]))),
+                                                __fmul2_rn(ts, make_float2(ws4[i], ws4[i])),
+                                                make_float2(bias4[i], bias4[i]));
+                    p[i] = pack2<T>(v.x, v.y);
+                  }
+                  // block i = lane / 8 (channels 8 i ..), token 8 j + lane % 8; 64-byte swizzle: 16-byte piece
+                  // i of token t lies at i ^ (t / 2 % 4)
+                  stmatrix_x4_trans(row + j * 512 + ((((lane >> 3) ^ (lane >> 1)) & 3) << 4), p[0], p[1], p[2], p[3]);
+                }
+              } else {
+                uint32_t r[16];
+                if (ok) {
+                  tmem_ld16(at, r);
+                  tmem_ld_wait();
+                }
+                if (c + CT >= c_end) drained();
+                __syncwarp();
+                const float2 w2 = make_float2(ws, ws), b2 = make_float2(bias, bias);
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                  const float4 ts = *reinterpret_cast<const float4*>(as + c + j);
+                  const float2 v0 = __ffma2_rn(make_float2(float(int(r[j])), float(int(r[j + 1]))),
+                                               __fmul2_rn(make_float2(ts.x, ts.y), w2), b2);
+                  const float2 v1 = __ffma2_rn(make_float2(float(int(r[j + 2])), float(int(r[j + 3]))),
+                                               __fmul2_rn(make_float2(ts.z, ts.w), w2), b2);
+                  const float v[4] = {v0.x, v0.y, v1.x, v1.y};
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)  // 128-byte swizzle: piece lane / 4 of token t lies at (lane / 4) ^ (t % 8)
+                    *reinterpret_cast<float*>(box + (j + e) * 128 + (((lane >> 2) ^ ((j + e) & 7)) << 4) +
+                                              (lane & 3) * 4) = v[e];
+                }
+              }
+              fence_proxy_async();
+              __syncwarp();
+              if (lane == 0) {
+                if (ok && x < a.N) tma_store_2d(&map_o, box, x, m0 + c);
+                bulk_commit();
+              }
+            }
+            if (half * (BT / 2) >= c_end) drained();
+          }
+        } else {
+          constexpr int CW = BT / 2 < 32 ? BT / 2 : 32;  // columns to a TMEM load
+#pragma unroll 1
+          for (int c = half * (BT / 2); ok && c < c_end; c += CW) {
             uint32_t r[CW];
             if constexpr (CW == 32) tmem_ld32(lane_base + uint32_t(b * BT + c), r);
             else if constexpr (CW == 16) tmem_ld16(lane_base + uint32_t(b * BT + c), r);
@@ -270,64 +378,51 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (MODE == PAIR) mbar_arrive_cluster(map_peer(&acc_empty[b], 0));
-          else mbar_arrive(&acc_empty[b]);
+          drained();
         }
       } else {
-        // partial sums to the CTA that finishes their token: token c to CTA c % split, slot c / split
-        const int slots = (BT + g.split - 1) / g.split;
-        if (ok) {
-          constexpr int CW = BT / 2 < 16 ? BT / 2 : 16;
+        // this CTA's partial sums, token by token, where the ring was (every load into it has been multiplied),
+        // and from there in one copy to each of the CTAs that finish them
+        int* part = reinterpret_cast<int*>(ring);
+        constexpr int CW = BT / 2 < 16 ? BT / 2 : 16;
 #pragma unroll 1
-          for (int c = half * (BT / 2); c < (half + 1) * (BT / 2) && c < mv; c += CW) {
-            uint32_t r[CW];
-            if constexpr (CW == 16) tmem_ld16(lane_base + uint32_t(c), r);
-            else tmem_ld8(lane_base + uint32_t(c), r);
-            tmem_ld_wait();
+        for (int c = half * (BT / 2); ok && c < (half + 1) * (BT / 2) && c < mv; c += CW) {
+          uint32_t r[CW];
+          if constexpr (CW == 16) tmem_ld16(lane_base + uint32_t(c), r);
+          else tmem_ld8(lane_base + uint32_t(c), r);
+          tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < CW; ++j) {
-              if (c + j < mv) {
-                const int owner = (c + j) % g.split, slot = (c + j) / g.split;
-                st_cluster_u32(map_peer(red + (int(rank) * slots + slot) * kChannels + ch, owner), r[j]);
-              }
+          for (int j = 0; j < CW; ++j) part[(c + j) * kChannels + ch] = int(r[j]);
+        }
+        fence_proxy_async();
+        named_bar(2, 32 * kEpi);
+        if (ok && et < g.split && et != int(rank)) {
+          const int count = max(0, min(run, mv - et * run));
+          if (count)
+            bulk_send(map_peer(red + int(rank) * run * kChannels, et), part + et * run * kChannels,
+                      uint32_t(count) * kChannels * 4, map_peer(red_full, et));
+        }
+        if (mine) {
+          if (!mbar_wait(red_full, 0, a.err, DEV_ERR_TIMEOUT_EPILOGUE)) ok = false;
+          if (ok && live) {
+            for (int t = half; t < mine; t += 2) {
+              const int c = int(rank) * run + t;
+              int sum = part[c * kChannels + ch];
+              for (int r = 0; r < g.split; ++r)
+                if (r != int(rank)) sum += red[(r * run + t) * kChannels + ch];
+              put(out + size_t(c) * a.ldo, fmaf(float(sum), as[c] * ws, bias));
             }
           }
         }
       }
     }
+    if (S::BOXES && lane == 0) bulk_wait_all();
   }
 
   __syncwarp();
-  if constexpr (MODE == SPLIT) {
-    tc_fence_before();
-    cluster_arrive_release();
-    cluster_wait_acquire();
-    tc_fence_after();
-    if (unit < tiles) {
-      int nt, mt;
-      tile_at(g, unit, nt, mt);
-      const int m0 = mt * BT, mv = min(BT, a.M - m0);
-      const int slots = (BT + g.split - 1) / g.split;
-      const int ch = tid & (kChannels - 1), n = nt * kChannels + ch;
-      if (tid < 2 * kChannels && n < a.N) {
-        const float ws = a.w_scale[n], bias = a.bias ? a.bias[n] : 0.0f;
-        for (int slot = tid / kChannels; slot * g.split + int(rank) < mv; slot += 2) {
-          const int c = slot * g.split + int(rank);
-          int sum = 0;
-          for (int r = 0; r < g.split; ++r) sum += red[(r * slots + slot) * kChannels + ch];
-          put(static_cast<T*>(a.out) + size_t(m0 + c) * a.ldo + n,
-              fmaf(float(sum), s_as[c] * ws, bias));
-        }
-      }
-    }
-  }
   tc_fence_before();
   __syncthreads();
-  if constexpr (MODE == PAIR) {  // neither CTA leaves while the other may still reach into it
+  if constexpr (MODE != ONE) {  // no CTA leaves while another may still reach into it
     cluster_arrive_release();
     cluster_wait_acquire();
   }
@@ -375,6 +470,11 @@ cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtenso
   g.tiles_m = (a.M + BT - 1) / BT;
   g.split = split;
   g.early_w = early_w;
+  CUtensorMap map_o = map_t;  // unused unless boxes
+  const size_t pitch = a.ldo * sizeof(T);
+  g.boxes = S::BOXES && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && pitch % 16 == 0;
+  if (g.boxes && make_tmap_store(&map_o, a.out, size_t(a.M), size_t(a.N), pitch, int(sizeof(T)), sizeof(T) == 4 ? 16 : 32))
+    return cudaErrorInvalidValue;
   const long long tiles = (long long)g.tiles_n * g.tiles_m;
   if (tiles > 0x7fffffffll / 16) return cudaErrorInvalidValue;
   const int cluster = MODE == PAIR ? 2 : split;
@@ -392,7 +492,7 @@ cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtenso
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = MODE == ONE ? 1 : 2;
-  return cudaLaunchKernelEx(&cfg, kernel, map_w, map_t, a, g);
+  return cudaLaunchKernelEx(&cfg, kernel, map_w, map_t, map_o, a, g);
 }
 
 struct Pick {

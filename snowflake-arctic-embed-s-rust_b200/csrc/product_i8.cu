@@ -97,7 +97,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* red_full = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, for the compiler too
   const uint32_t rank = MODE == ONE ? 0u : cluster_ctarank();
   const int unit = int(blockIdx.x) / (MODE == PAIR ? 2 : g.split);          // tile walker
   const int units = int(gridDim.x) / (MODE == PAIR ? 2 : g.split);
@@ -140,20 +141,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the first blocks of weights are asked for before the kernel ahead (which quantizes the tokens) has ended
   int early = 0;
   if (g.early_w) {
-    if (warp == 0 && lane == 0 && unit < tiles) {
+    if (warp == 0 && unit < tiles) {
       int nt, mt;
       tile_at(g, unit, nt, mt);
       uint32_t lead = 0;
       if constexpr (MODE == PAIR) lead = map_peer(full, 0);
-      for (; early < STAGES && kb0 + early < kb1; ++early) {
-        uint8_t* st = ring + early * S::STAGE;
-        if constexpr (MODE == PAIR) {
-          if (rank == 0) mbar_arrive_expect_tx(&full[early], 2 * S::STAGE);
-          tma_load_2d_pair(st, &map_w, lead + 8 * early, (kb0 + early) * kBlock, (nt * 2 + int(rank)) * kChannels);
-        } else {
-          mbar_arrive_expect_tx(&full[early], S::STAGE);
-          tma_load_2d(st, &map_w, &full[early], (kb0 + early) * kBlock, nt * kChannels);
+      early = min(STAGES, kb1 - kb0);
+      for (int s = 0; s < early; ++s) {
+        uint8_t* st = ring + s * S::STAGE;
+        if (elect_one()) {
+          if constexpr (MODE == PAIR) {
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::STAGE);
+            tma_load_2d_pair(st, &map_w, lead + 8 * s, (kb0 + s) * kBlock, (nt * 2 + int(rank)) * kChannels);
+          } else {
+            mbar_arrive_expect_tx(&full[s], S::STAGE);
+            tma_load_2d(st, &map_w, &full[s], (kb0 + s) * kBlock, nt * kChannels);
+          }
         }
+        __syncwarp();
       }
     }
     pdl_wait();
@@ -178,70 +183,77 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer
-    if (lane == 0) {
-      uint32_t lead = 0;
-      if constexpr (MODE == PAIR) lead = map_peer(full, 0);
-      bool ok = true;
-      int kc = 0;
-      for (int tile = unit; tile < tiles && ok; tile += units) {
-        int nt, mt;
-        tile_at(g, tile, nt, mt);
-        for (int kb = kb0; kb < kb1; ++kb, ++kc) {
-          const int s = kc % STAGES;
-          if (kc >= STAGES && !(ok = mbar_wait(&empty[s], ((kc / STAGES) - 1) & 1, a.err, DEV_ERR_TIMEOUT_PRODUCER)))
-            break;
-          uint8_t* st = ring + s * S::STAGE;
+    uint32_t lead = 0;
+    if constexpr (MODE == PAIR) lead = map_peer(full, 0);
+    bool ok = true;
+    int kc = 0, s = 0;
+    uint32_t phase = 1;  // of the ring's last round; its first finds every stage empty
+    for (int tile = unit; tile < tiles && ok; tile += units) {
+      int nt, mt;
+      tile_at(g, tile, nt, mt);
+      const int wy = (nt * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels;
+      const int ty = mt * BT + (MODE == PAIR ? int(rank) * (BT / 2) : 0);
+      for (int kb = kb0; kb < kb1; ++kb, ++kc) {
+        if (kc >= STAGES && !(ok = mbar_wait_warp(&empty[s], phase, a.err, DEV_ERR_TIMEOUT_PRODUCER))) break;
+        uint8_t* st = ring + s * S::STAGE;
+        if (elect_one()) {
           if constexpr (MODE == PAIR) {
             if (kc >= early) {
               if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * S::STAGE);
-              tma_load_2d_pair(st, &map_w, lead + 8 * s, kb * kBlock, (nt * 2 + int(rank)) * kChannels);
+              tma_load_2d_pair(st, &map_w, lead + 8 * s, kb * kBlock, wy);
             }
-            tma_load_2d_pair(st + S::W_BYTES, &map_t, lead + 8 * s, kb * kBlock, mt * BT + int(rank) * (BT / 2));
+            tma_load_2d_pair(st + S::W_BYTES, &map_t, lead + 8 * s, kb * kBlock, ty);
           } else {
             if (kc >= early) {
               mbar_arrive_expect_tx(&full[s], S::STAGE);
-              tma_load_2d(st, &map_w, &full[s], kb * kBlock, nt * kChannels);
+              tma_load_2d(st, &map_w, &full[s], kb * kBlock, wy);
             }
-            tma_load_2d(st + S::W_BYTES, &map_t, &full[s], kb * kBlock, mt * BT);
+            tma_load_2d(st + S::W_BYTES, &map_t, &full[s], kb * kBlock, ty);
           }
         }
+        __syncwarp();
+        if (++s == STAGES) s = 0, phase ^= 1;
       }
-      // no load is in flight when the CTA ends, even where the MMAs gave up waiting for one
-      if (MODE != PAIR || rank == 0)
-        for (int i = max(0, kc - STAGES); i < kc; ++i)
-          mbar_wait(&full[i % STAGES], (i / STAGES) & 1, a.err, DEV_ERR_TIMEOUT_PRODUCER);
     }
+    // no load is in flight when the CTA ends, even where the MMAs gave up waiting for one
+    if (MODE != PAIR || rank == 0)
+      for (int i = max(0, kc - STAGES); i < kc; ++i)
+        mbar_wait(&full[i % STAGES], (i / STAGES) & 1, a.err, DEV_ERR_TIMEOUT_PRODUCER);
     __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------ MMA issuer (CTA 0 of a pair issues for both)
-    if (lane == 0 && (MODE != PAIR || rank == 0)) {
+    if (MODE != PAIR || rank == 0) {
       constexpr uint32_t idesc = idesc_i8(kChannels * CG, BT);
       bool ok = true;
-      int kc = 0, it = 0;
+      int it = 0, s = 0;
+      uint32_t phase = 0;
       for (int tile = unit; tile < tiles && ok; tile += units, ++it) {
         const int b = it & 1, u = it >> 1;
-        if (u >= 1 && !(ok = mbar_wait(&acc_empty[b], (u - 1) & 1, a.err, DEV_ERR_TIMEOUT_MMA))) break;
+        if (u >= 1 && !(ok = mbar_wait_warp(&acc_empty[b], (u - 1) & 1, a.err, DEV_ERR_TIMEOUT_MMA))) break;
         tc_fence_after();
         const uint32_t d = tmem + uint32_t(b * BT);
-        for (int kb = kb0; kb < kb1; ++kb, ++kc) {
-          const int s = kc % STAGES;
-          if (!(ok = mbar_wait(&full[s], (kc / STAGES) & 1, a.err, DEV_ERR_TIMEOUT_MMA))) break;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!(ok = mbar_wait_warp(&full[s], phase, a.err, DEV_ERR_TIMEOUT_MMA))) break;
           tc_fence_after();
-          const uint32_t w_addr = smem_u32(ring + s * S::STAGE), t_addr = w_addr + S::W_BYTES;
+          const uint64_t wd = sdesc_sw128(smem_u32(ring) + uint32_t(s) * S::STAGE);
+          const uint64_t td = wd + (S::W_BYTES >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kBlock / 32; ++ks) {
-            const uint32_t more = kb > kb0 || ks > 0;
-            if constexpr (MODE == PAIR)
-              mma_i8_pair(d, sdesc_sw128(w_addr + ks * 32), sdesc_sw128(t_addr + ks * 32), idesc, more);
-            else
-              mma_i8(d, sdesc_sw128(w_addr + ks * 32), sdesc_sw128(t_addr + ks * 32), idesc, more);
+            for (int ks = 0; ks < kBlock / 32; ++ks) {  // 32 bytes on: + 2 in the descriptors' address field
+              const uint32_t more = kb > kb0 || ks > 0;
+              if constexpr (MODE == PAIR) mma_i8_pair(d, wd + 2 * ks, td + 2 * ks, idesc, more);
+              else mma_i8(d, wd + 2 * ks, td + 2 * ks, idesc, more);
+            }
+            if constexpr (MODE == PAIR) {
+              mma_commit_pair(&empty[s]);
+              if (kb == kb1 - 1) mma_commit_pair(&acc_full[b]);
+            } else {
+              mma_commit(&empty[s]);
+              if (kb == kb1 - 1) mma_commit(&acc_full[b]);
+            }
           }
-          if constexpr (MODE == PAIR) mma_commit_pair(&empty[s]);
-          else mma_commit(&empty[s]);
-        }
-        if (ok) {
-          if constexpr (MODE == PAIR) mma_commit_pair(&acc_full[b]);
-          else mma_commit(&acc_full[b]);
+          __syncwarp();
+          if (++s == STAGES) s = 0, phase ^= 1;
         }
       }
     }

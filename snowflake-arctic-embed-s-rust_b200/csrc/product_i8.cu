@@ -12,7 +12,8 @@
 //   warp 0      TMA producer: 128-byte depth blocks of both operands into a ring (128-byte swizzle; bytes past
 //               the depth, rows past the operands' ends are filled with zeros by the copy)
 //   warp 1      one thread issues the MMAs into one of two TMEM accumulators taken in turn
-//   warps 2-9   epilogue, two warps to a lane quadrant, half of the tokens each; overlaps the next tile's MMAs
+//   warps 2-17  epilogue, four warps to a lane quadrant, a quarter of the tokens each; overlaps the next tile's
+//               MMAs (with 8 warps the TMEM and shared-memory latencies showed)
 // Variants:
 //   PAIR   two CTAs hold a 256-channel tile (cta_group::2): each stages 128 channels and half of the tokens, a
 //          third less L2 traffic a product at 256 tokens, where that traffic is what one CTA alone waits for.
@@ -33,12 +34,16 @@ namespace {
 
 constexpr int kChannels = 128;                 // weight rows to a CTA
 constexpr int kBlock = 128;                    // depth bytes to a ring stage
-constexpr int kEpi = 8;                        // epilogue warps
+constexpr int kEpi = 16;                       // epilogue warps
 constexpr int kThreads = 32 * (2 + kEpi);
 constexpr int kSmemMost = 232448;
 constexpr int kMaxSplit = 8;
-constexpr int kBoxBytes = 2048;                // one box of results: 32 channels x 32 (16-bit) or 16 (float) tokens
+constexpr int kBoxBytes = 2048;                // a warp's box of results: 32 channels x kBoxTokens
 constexpr int kGroupM = 8;                     // token tiles walked together, for L2 reuse of the weights
+
+// Tokens to a box: 32 of 16-bit results (16 where a warp has no more), 16 of float.
+template <class T, int BT>
+constexpr int kBoxTokens = sizeof(T) == 4 || BT == 64 ? 16 : 32;
 
 enum Mode { ONE = 0, PAIR = 1, SPLIT = 2 };
 
@@ -50,8 +55,9 @@ struct Shape {
   static constexpr int STAGE = W_BYTES + T_BYTES;
   static constexpr int RED = MODE == SPLIT ? (BT + kMaxSplit) * kChannels * 4 : 0;  // partial sums sent here
   static constexpr bool BOXES = MODE != SPLIT && BT >= 64;    // results leave as boxes where the output allows
-  static constexpr int OUT = BOXES ? kEpi * 2 * kBoxBytes : 0;
-  static constexpr int FIXED = OUT + RED + 2 * BT * 4 + 256;
+  static constexpr int OUT = BOXES ? kEpi * kBoxBytes : 0;
+  static constexpr int PARAM = 2 * kChannels + BT;            // w_scale, bias and token scales of a tile
+  static constexpr int FIXED = OUT + RED + 2 * PARAM * 4 + 256;
   static constexpr int FIT = (kSmemMost - FIXED) / STAGE;
   static constexpr int STAGES = FIT < 12 ? FIT : 12;
   static constexpr int TOTAL = FIXED + STAGES * STAGE;
@@ -75,6 +81,14 @@ __device__ __forceinline__ void tile_at(const Grid& g, int tile, int& nt, int& m
   nt = r / gm;
 }
 
+template <int W>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[W]) {
+  if constexpr (W == 32) tmem_ld32(at, r);
+  else if constexpr (W == 16) tmem_ld16(at, r);
+  else if constexpr (W == 8) tmem_ld8(at, r);
+  else tmem_ld4(at, r);
+}
+
 template <class T>
 __device__ __forceinline__ void put(T* p, float v) { *p = from_f32<T>(v); }
 
@@ -89,8 +103,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = smem_product;
   uint8_t* s_out = ring + STAGES * S::STAGE;
   int* red = reinterpret_cast<int*>(s_out + S::OUT);
-  float* s_as = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // [2][BT] token scales
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_as + 2 * BT);
+  float* s_param = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // two tiles'
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_param + 2 * S::PARAM);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
@@ -260,14 +274,24 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------ epilogue
-    const int et = tid - 64;                 // 0..255
-    const int half = (warp - 2) >> 2;        // which half of the tokens
+    const int et = tid - 64;                 // 0..511
+    const int part4 = (warp - 2) >> 2;       // which quarter of the tokens
+    constexpr int QW = BT / 4;               // tokens to a quarter
     const int ch = (warp & 3) * 32 + lane;   // channel within the CTA's 128 = TMEM lane
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+    // a tile's scales and biases, a value a thread, asked for a tile ahead
+    auto fetch = [&](int tile) {
+      int nt, mt;
+      tile_at(g, tile, nt, mt);
+      const int n = (nt * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + (et & (kChannels - 1));
+      const int m = mt * BT + et - 2 * kChannels;
+      if (et < kChannels) return n < a.N ? a.w_scale[n] : 0.0f;
+      if (et < 2 * kChannels) return n < a.N && a.bias ? a.bias[n] : 0.0f;
+      return et < S::PARAM && m < a.M ? a.a_scale[m] : 0.0f;
+    };
+    float param = unit < tiles ? fetch(unit) : 0.0f;
     bool ok = true;
     int it = 0;
-    [[maybe_unused]] int turn = 0;                  // which of the warp's two boxes
-    [[maybe_unused]] float ws4[4], bias4[4];
     for (int tile = unit; tile < tiles; tile += units, ++it) {
       const int b = it & 1, u = it >> 1;
       int nt, mt;
@@ -276,17 +300,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int m0 = mt * BT;
       const int mv = min(BT, a.M - m0);      // tokens of this tile
       const bool live = n < a.N;
-      float* as = s_as + b * BT;
-      if (et < mv) as[et] = a.a_scale[m0 + et];
-      const float ws = live ? a.w_scale[n] : 0.0f;
-      const float bias = live && a.bias ? a.bias[n] : 0.0f;
-      T* out = static_cast<T*>(a.out) + size_t(m0) * a.ldo + n;
-      named_bar(2, 32 * kEpi);               // the scales are there; the other buffer's readers are done
+      float* s_ws = s_param + b * S::PARAM;
+      const float* s_bias = s_ws + kChannels;
+      const float* as = s_bias + kChannels;
+      if (et < S::PARAM) s_ws[et] = param;
+      if (tile + units < tiles) param = fetch(tile + units);
+      named_bar(2, 32 * kEpi);               // they are there; the other buffer's readers are done
       if (ok) ok = mbar_wait(&acc_full[b], u & 1, a.err, DEV_ERR_TIMEOUT_EPILOGUE);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+      const int c0 = part4 * QW;
+      const float ws = s_ws[ch], bias = s_bias[ch];
+      T* out = static_cast<T*>(a.out) + size_t(m0) * a.ldo + n;
       if constexpr (MODE != SPLIT) {
-        const int c_end = min(mv, (half + 1) * (BT / 2));
+        const int c_end = min(mv, c0 + QW);
         auto drained = [&] {  // this warp has read its part of the accumulator
           tc_fence_before();
           __syncwarp();
@@ -297,35 +324,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (S::BOXES && g.boxes) {
           if constexpr (S::BOXES) {
-            uint8_t* box0 = s_out + (warp - 2) * 2 * kBoxBytes;
+            uint8_t* box = s_out + (warp - 2) * kBoxBytes;
             const int x = n - lane;
-            constexpr int CT = sizeof(T) == 4 ? 16 : 32;
-            if constexpr (sizeof(T) == 2) {
-              // fragment lanes: channel lane / 4 + 8 i, i = 0..3
+            constexpr int CT = kBoxTokens<T, BT>;
+            [[maybe_unused]] float ws4[4], bias4[4];
+            if constexpr (sizeof(T) == 2) {  // the fragments' lanes: channels lane / 4 + 8 i
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int ni = x + (lane >> 2) + 8 * i;
-                ws4[i] = ni < a.N ? a.w_scale[ni] : 0.0f;
-                bias4[i] = ni < a.N && a.bias ? a.bias[ni] : 0.0f;
+                ws4[i] = s_ws[ch - lane + (lane >> 2) + 8 * i];
+                bias4[i] = s_bias[ch - lane + (lane >> 2) + 8 * i];
               }
             }
 #pragma unroll 1
-            for (int c = half * (BT / 2); c < c_end; c += CT, turn ^= 1) {
-              uint8_t* box = box0 + turn * kBoxBytes;
+            for (int c = c0; c < c_end; c += CT) {
               const uint32_t at = lane_base + uint32_t(b * BT + c);
-              if (lane == 0) bulk_wait_read<1>();  // the store that left from this box two turns ago
               if constexpr (sizeof(T) == 2) {
-                uint32_t lo[16], hi[16];
+                uint32_t lo[CT / 2], hi[CT / 2];
                 if (ok) {
-                  tmem_ld_16x32(at, lo);
-                  tmem_ld_16x32(at + (16u << 16), hi);
+                  if constexpr (CT == 32) {
+                    tmem_ld_16x32(at, lo);
+                    tmem_ld_16x32(at + (16u << 16), hi);
+                  } else {
+                    tmem_ld_16x16(at, lo);
+                    tmem_ld_16x16(at + (16u << 16), hi);
+                  }
                   tmem_ld_wait();
                 }
                 if (c + CT >= c_end) drained();
+                if (lane == 0) bulk_wait_read<0>();  // the box's last store has left
                 __syncwarp();
                 const uint32_t row = smem_u32(box) + (lane & 7) * 64;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < CT / 8; ++j) {
                   const float2 ts = *reinterpret_cast<const float2*>(as + c + 8 * j + 2 * (lane & 3));
                   uint32_t p[4];
 #pragma unroll
@@ -347,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   tmem_ld_wait();
                 }
                 if (c + CT >= c_end) drained();
+                if (lane == 0) bulk_wait_read<0>();
                 __syncwarp();
                 const float2 w2 = make_float2(ws, ws), b2 = make_float2(bias, bias);
 #pragma unroll
@@ -370,16 +401,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bulk_commit();
               }
             }
-            if (half * (BT / 2) >= c_end) drained();
+            if (c0 >= c_end) drained();
           }
         } else {
-          constexpr int CW = BT / 2 < 32 ? BT / 2 : 32;  // columns to a TMEM load
+          constexpr int CW = QW < 32 ? QW : 32;  // columns to a TMEM load
 #pragma unroll 1
-          for (int c = half * (BT / 2); ok && c < c_end; c += CW) {
+          for (int c = c0; ok && c < c_end; c += CW) {
             uint32_t r[CW];
-            if constexpr (CW == 32) tmem_ld32(lane_base + uint32_t(b * BT + c), r);
-            else if constexpr (CW == 16) tmem_ld16(lane_base + uint32_t(b * BT + c), r);
-            else tmem_ld8(lane_base + uint32_t(b * BT + c), r);
+            tmem_ld_cols<CW>(lane_base + uint32_t(b * BT + c), r);
             tmem_ld_wait();
             T* p = out + size_t(c) * a.ldo;
             if (live) {
@@ -396,15 +425,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         // this CTA's partial sums, token by token, where the ring was (every load into it has been multiplied),
         // and from there in one copy to each of the CTAs that finish them
         int* part = reinterpret_cast<int*>(ring);
-        constexpr int CW = BT / 2 < 16 ? BT / 2 : 16;
-#pragma unroll 1
-        for (int c = half * (BT / 2); ok && c < (half + 1) * (BT / 2) && c < mv; c += CW) {
-          uint32_t r[CW];
-          if constexpr (CW == 16) tmem_ld16(lane_base + uint32_t(c), r);
-          else tmem_ld8(lane_base + uint32_t(c), r);
+        if (ok && c0 < mv) {
+          uint32_t r[QW];
+          tmem_ld_cols<QW>(lane_base + uint32_t(c0), r);
           tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < CW; ++j) part[(c + j) * kChannels + ch] = int(r[j]);
+          for (int j = 0; j < QW; ++j) part[(c0 + j) * kChannels + ch] = int(r[j]);
         }
         fence_proxy_async();
         named_bar(2, 32 * kEpi);
@@ -417,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (mine) {
           if (!mbar_wait(red_full, 0, a.err, DEV_ERR_TIMEOUT_EPILOGUE)) ok = false;
           if (ok && live) {
-            for (int t = half; t < mine; t += 2) {
+            for (int t = part4; t < mine; t += 4) {
               const int c = int(rank) * run + t;
               int sum = part[c * kChannels + ch];
               for (int r = 0; r < g.split; ++r)
@@ -485,7 +511,7 @@ cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtenso
   CUtensorMap map_o = map_t;  // unused unless boxes
   const size_t pitch = a.ldo * sizeof(T);
   g.boxes = S::BOXES && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && pitch % 16 == 0;
-  if (g.boxes && make_tmap_store(&map_o, a.out, size_t(a.M), size_t(a.N), pitch, int(sizeof(T)), sizeof(T) == 4 ? 16 : 32))
+  if (g.boxes && make_tmap_store(&map_o, a.out, size_t(a.M), size_t(a.N), pitch, int(sizeof(T)), kBoxTokens<T, BT>))
     return cudaErrorInvalidValue;
   const long long tiles = (long long)g.tiles_n * g.tiles_m;
   if (tiles > 0x7fffffffll / 16) return cudaErrorInvalidValue;

@@ -56,8 +56,7 @@ struct Shape {
   static constexpr int RED = MODE == SPLIT ? (BT + kMaxSplit) * kChannels * 4 : 0;  // partial sums sent here
   static constexpr bool BOXES = MODE != SPLIT && BT >= 64;    // results leave as boxes where the output allows
   static constexpr int OUT = BOXES ? kEpi * kBoxBytes : 0;
-  static constexpr int PARAM = 2 * kChannels + BT;            // w_scale, bias and token scales of a tile
-  static constexpr int FIXED = OUT + RED + 2 * PARAM * 4 + 256;
+  static constexpr int FIXED = OUT + RED + kEpi * 32 * 4 + 256;
   static constexpr int FIT = (kSmemMost - FIXED) / STAGE;
   static constexpr int STAGES = FIT < 12 ? FIT : 12;
   static constexpr int TOTAL = FIXED + STAGES * STAGE;
@@ -72,14 +71,27 @@ struct Grid {
   int boxes;     // store results as TMA boxes (the output's base and pitch are multiples of 16 bytes)
 };
 
-__device__ __forceinline__ void tile_at(const Grid& g, int tile, int& nt, int& mt) {
-  const int per = kGroupM * g.tiles_n;
-  const int first = tile / per * kGroupM;
-  const int gm = min(kGroupM, g.tiles_m - first);
-  const int r = tile % per;
-  mt = first + r % gm;
-  nt = r / gm;
-}
+// The tiles a CTA (or pair, or cluster) takes, `units` apart in an order that walks the channels of kGroupM token
+// tiles at a time. Divides only where a step leaves such a group.
+struct Walk {
+  int r, first, per, gm;
+  __device__ __forceinline__ Walk(const Grid& g, int tile) : r(tile), first(0), per(kGroupM * g.tiles_n) { settle(g); }
+  __device__ __forceinline__ void step(const Grid& g, int units) {
+    r += units;
+    settle(g);
+  }
+  __device__ __forceinline__ void settle(const Grid& g) {
+    if (r >= per) {
+      const int q = r / per;
+      r -= q * per;
+      first += q * kGroupM;
+    }
+    gm = min(kGroupM, g.tiles_m - first);
+  }
+  __device__ __forceinline__ bool more(const Grid& g) const { return gm > 0 && r < gm * g.tiles_n; }
+  __device__ __forceinline__ int nt() const { return gm == kGroupM ? r / kGroupM : r / gm; }
+  __device__ __forceinline__ int mt() const { return first + (gm == kGroupM ? r % kGroupM : r % gm); }
+};
 
 template <int W>
 __device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[W]) {
@@ -103,8 +115,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = smem_product;
   uint8_t* s_out = ring + STAGES * S::STAGE;
   int* red = reinterpret_cast<int*>(s_out + S::OUT);
-  float* s_param = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // two tiles'
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_param + 2 * S::PARAM);
+  float* s_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // 32 tokens' to a warp
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + kEpi * 32);
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
@@ -116,7 +128,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = MODE == ONE ? 0u : cluster_ctarank();
   const int unit = int(blockIdx.x) / (MODE == PAIR ? 2 : g.split);          // tile walker
   const int units = int(gridDim.x) / (MODE == PAIR ? 2 : g.split);
-  const int tiles = g.tiles_n * g.tiles_m;
   const int KB = (a.K + kBlock - 1) / kBlock;
   const int kb0 = MODE == SPLIT ? int((long long)(KB) * rank / g.split) : 0;
   const int kb1 = MODE == SPLIT ? int((long long)(KB) * (rank + 1) / g.split) : KB;
@@ -138,9 +149,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   // SPLIT: the tile's tokens are finished in runs of `run`, CTA r taking `mine` of them from token r * run on
   int run = 0, mine = 0;
   if constexpr (MODE == SPLIT) {
-    int nt, mt;
-    tile_at(g, unit, nt, mt);
-    const int mv = min(BT, a.M - mt * BT);
+    const Walk w(g, unit);
+    const int mv = min(BT, a.M - w.mt() * BT);
     run = (mv + g.split - 1) / g.split;
     mine = max(0, min(run, mv - int(rank) * run));
     if (tid == 0 && mine) mbar_arrive_expect_tx(red_full, uint32_t(g.split - 1) * mine * kChannels * 4);
@@ -155,9 +165,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the first blocks of weights are asked for before the kernel ahead (which quantizes the tokens) has ended
   int early = 0;
   if (g.early_w) {
-    if (warp == 0 && unit < tiles) {
-      int nt, mt;
-      tile_at(g, unit, nt, mt);
+    const Walk w(g, unit);
+    if (warp == 0 && w.more(g)) {
+      const int nt = w.nt();
       uint32_t lead = 0;
       if constexpr (MODE == PAIR) lead = map_peer(full, 0);
       early = min(STAGES, kb1 - kb0);
@@ -202,11 +212,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int kc = 0, s = 0;
     uint32_t phase = 1;  // of the ring's last round; its first finds every stage empty
-    for (int tile = unit; tile < tiles && ok; tile += units) {
-      int nt, mt;
-      tile_at(g, tile, nt, mt);
-      const int wy = (nt * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels;
-      const int ty = mt * BT + (MODE == PAIR ? int(rank) * (BT / 2) : 0);
+    for (Walk w(g, unit); w.more(g) && ok; w.step(g, units)) {
+      const int wy = (w.nt() * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels;
+      const int ty = w.mt() * BT + (MODE == PAIR ? int(rank) * (BT / 2) : 0);
       for (int kb = kb0; kb < kb1; ++kb, ++kc) {
         if (kc >= STAGES && !(ok = mbar_wait_warp(&empty[s], phase, a.err, DEV_ERR_TIMEOUT_PRODUCER))) break;
         uint8_t* st = ring + s * S::STAGE;
@@ -241,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int it = 0, s = 0;
       uint32_t phase = 0;
-      for (int tile = unit; tile < tiles && ok; tile += units, ++it) {
+      for (Walk w(g, unit); w.more(g) && ok; w.step(g, units), ++it) {
         const int b = it & 1, u = it >> 1;
         if (u >= 1 && !(ok = mbar_wait_warp(&acc_empty[b], (u - 1) & 1, a.err, DEV_ERR_TIMEOUT_MMA))) break;
         tc_fence_after();
@@ -279,38 +287,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int QW = BT / 4;               // tokens to a quarter
     const int ch = (warp & 3) * 32 + lane;   // channel within the CTA's 128 = TMEM lane
     const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-    // a tile's scales and biases, a value a thread, asked for a tile ahead
-    auto fetch = [&](int tile) {
-      int nt, mt;
-      tile_at(g, tile, nt, mt);
-      const int n = (nt * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + (et & (kChannels - 1));
-      const int m = mt * BT + et - 2 * kChannels;
-      if (et < kChannels) return n < a.N ? a.w_scale[n] : 0.0f;
-      if (et < 2 * kChannels) return n < a.N && a.bias ? a.bias[n] : 0.0f;
-      return et < S::PARAM && m < a.M ? a.a_scale[m] : 0.0f;
+    const int c0 = part4 * QW;
+    float* as = s_scale + (warp - 2) * 32;   // scales of the 32 tokens at hand
+    // Each warp keeps its own scales and biases: a lane's channel's, and those of tokens lane and lane + 32 of
+    // its quarter, asked for a tile ahead. Warps meet only at the accumulators' barriers, so that one's TMEM
+    // and shared-memory latencies pass under another's arithmetic.
+    constexpr int TW = (QW + 31) / 32;
+    float ws_next, bias_next, as_next[TW];
+    int n_next = 0, m_next = 0;
+    Walk w(g, unit);
+    auto fetch = [&] {
+      n_next = (w.nt() * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + ch;
+      m_next = w.mt() * BT;
+      ws_next = n_next < a.N ? a.w_scale[n_next] : 0.0f;
+      bias_next = n_next < a.N && a.bias ? a.bias[n_next] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < TW; ++i) {
+        const int t = lane + 32 * i, m = m_next + c0 + t;
+        as_next[i] = t < QW && m < a.M ? a.a_scale[m] : 0.0f;
+      }
     };
-    float param = unit < tiles ? fetch(unit) : 0.0f;
+    bool more = w.more(g);
+    if (more) fetch();
     bool ok = true;
     int it = 0;
-    for (int tile = unit; tile < tiles; tile += units, ++it) {
+    for (; more; ++it) {
       const int b = it & 1, u = it >> 1;
-      int nt, mt;
-      tile_at(g, tile, nt, mt);
-      const int n = (nt * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + ch;
-      const int m0 = mt * BT;
+      const int n = n_next, m0 = m_next;
       const int mv = min(BT, a.M - m0);      // tokens of this tile
       const bool live = n < a.N;
-      float* s_ws = s_param + b * S::PARAM;
-      const float* s_bias = s_ws + kChannels;
-      const float* as = s_bias + kChannels;
-      if (et < S::PARAM) s_ws[et] = param;
-      if (tile + units < tiles) param = fetch(tile + units);
-      named_bar(2, 32 * kEpi);               // they are there; the other buffer's readers are done
+      const float ws = ws_next, bias = bias_next;
+      float as_own[TW];
+#pragma unroll
+      for (int i = 0; i < TW; ++i) as_own[i] = as_next[i];
+      w.step(g, units);
+      more = w.more(g);
+      if (more) fetch();
       if (ok) ok = mbar_wait(&acc_full[b], u & 1, a.err, DEV_ERR_TIMEOUT_EPILOGUE);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
-      const int c0 = part4 * QW;
-      const float ws = s_ws[ch], bias = s_bias[ch];
+      // before the columns from c on: the scales of their 32 tokens
+      auto scales = [&](int c) {
+        if (((c - c0) & 31) == 0) {
+          __syncwarp();
+          as[lane] = TW == 1 || c == c0 ? as_own[0] : as_own[TW - 1];
+          __syncwarp();
+        }
+      };
       T* out = static_cast<T*>(a.out) + size_t(m0) * a.ldo + n;
       if constexpr (MODE != SPLIT) {
         const int c_end = min(mv, c0 + QW);
@@ -331,13 +354,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (sizeof(T) == 2) {  // the fragments' lanes: channels lane / 4 + 8 i
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                ws4[i] = s_ws[ch - lane + (lane >> 2) + 8 * i];
-                bias4[i] = s_bias[ch - lane + (lane >> 2) + 8 * i];
+                ws4[i] = __shfl_sync(0xffffffffu, ws, (lane >> 2) + 8 * i);
+                bias4[i] = __shfl_sync(0xffffffffu, bias, (lane >> 2) + 8 * i);
               }
             }
 #pragma unroll 1
             for (int c = c0; c < c_end; c += CT) {
               const uint32_t at = lane_base + uint32_t(b * BT + c);
+              scales(c);
+              const float* cs = as + ((c - c0) & 31);
               if constexpr (sizeof(T) == 2) {
                 uint32_t lo[CT / 2], hi[CT / 2];
                 if (ok) {
@@ -356,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t row = smem_u32(box) + (lane & 7) * 64;
 #pragma unroll
                 for (int j = 0; j < CT / 8; ++j) {
-                  const float2 ts = *reinterpret_cast<const float2*>(as + c + 8 * j + 2 * (lane & 3));
+                  const float2 ts = *reinterpret_cast<const float2*>(cs + 8 * j + 2 * (lane & 3));
                   uint32_t p[4];
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
@@ -382,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float2 w2 = make_float2(ws, ws), b2 = make_float2(bias, bias);
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                  const float4 ts = *reinterpret_cast<const float4*>(as + c + j);
+                  const float4 ts = *reinterpret_cast<const float4*>(cs + j);
                   const float2 v0 = __ffma2_rn(make_float2(float(int(r[j])), float(int(r[j + 1]))),
                                                __fmul2_rn(make_float2(ts.x, ts.y), w2), b2);
                   const float2 v1 = __ffma2_rn(make_float2(float(int(r[j + 2])), float(int(r[j + 3]))),
@@ -408,13 +433,14 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
           for (int c = c0; ok && c < c_end; c += CW) {
             uint32_t r[CW];
+            scales(c);
             tmem_ld_cols<CW>(lane_base + uint32_t(b * BT + c), r);
             tmem_ld_wait();
             T* p = out + size_t(c) * a.ldo;
             if (live) {
 #pragma unroll
               for (int j = 0; j < CW; ++j) {
-                if (c + j < mv) put(p, fmaf(float(int(r[j])), as[c + j] * ws, bias));
+                if (c + j < mv) put(p, fmaf(float(int(r[j])), as[j] * ws, bias));
                 p += a.ldo;
               }
             }
@@ -448,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               int sum = part[c * kChannels + ch];
               for (int r = 0; r < g.split; ++r)
                 if (r != int(rank)) sum += red[(r * run + t) * kChannels + ch];
-              put(out + size_t(c) * a.ldo, fmaf(float(sum), as[c] * ws, bias));
+              put(out + size_t(c) * a.ldo, fmaf(float(sum), a.a_scale[m0 + c] * ws, bias));
             }
           }
         }

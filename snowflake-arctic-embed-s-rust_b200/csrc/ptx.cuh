@@ -392,9 +392,11 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
-// Arrive on a barrier anywhere in the cluster (addr from map_peer).
+// Arrive on a barrier anywhere in the cluster (addr from map_peer), after this thread's TMEM loads (tc_fence_before)
+// but ordering none of its memory writes for the other CTA: a release at cluster scope waits for stores and
+// bulk stores in flight (measured: 2,000 cycles behind a box of results).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_addr) : "memory");
 }
 
 // ---------------------------------------------------------------- clusters

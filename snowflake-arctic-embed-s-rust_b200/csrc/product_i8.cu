@@ -39,7 +39,6 @@ constexpr int kThreads = 32 * (2 + kEpi);
 constexpr int kSmemMost = 232448;
 constexpr int kMaxSplit = 8;
 constexpr int kBoxBytes = 2048;                // a warp's box of results: 32 channels x kBoxTokens
-constexpr int kGroupM = 8;                     // token tiles walked together, for L2 reuse of the weights
 
 // Tokens to a box: 32 of 16-bit results (16 where a warp has no more), 16 of float.
 template <class T, int BT>
@@ -68,14 +67,18 @@ struct Grid {
   int tiles_n, tiles_m;
   int split;     // CTAs that share a tile's depth
   int early_w;   // the weights may be read before the kernel ahead has ended
+  int group;     // log2 of the token tiles walked together
   int boxes;     // store results as TMA boxes (the output's base and pitch are multiples of 16 bytes)
 };
 
-// The tiles a CTA (or pair, or cluster) takes, `units` apart in an order that walks the channels of kGroupM token
+// The tiles a CTA (or pair, or cluster) takes, `units` apart in an order that walks the channels of 1 << group token
 // tiles at a time. Divides only where a step leaves such a group.
 struct Walk {
-  int r, first, per, gm;
-  __device__ __forceinline__ Walk(const Grid& g, int tile) : r(tile), first(0), per(kGroupM * g.tiles_n) { settle(g); }
+  int r, first, per, gm, full;
+  __device__ __forceinline__ Walk(const Grid& g, int tile)
+      : r(tile), first(0), per(g.tiles_n << g.group), full(1 << g.group) {
+    settle(g);
+  }
   __device__ __forceinline__ void step(const Grid& g, int units) {
     r += units;
     settle(g);
@@ -84,13 +87,13 @@ struct Walk {
     if (r >= per) {
       const int q = r / per;
       r -= q * per;
-      first += q * kGroupM;
+      first += q << g.group;
     }
-    gm = min(kGroupM, g.tiles_m - first);
+    gm = min(full, g.tiles_m - first);
   }
   __device__ __forceinline__ bool more(const Grid& g) const { return gm > 0 && r < gm * g.tiles_n; }
-  __device__ __forceinline__ int nt() const { return gm == kGroupM ? r / kGroupM : r / gm; }
-  __device__ __forceinline__ int mt() const { return first + (gm == kGroupM ? r % kGroupM : r % gm); }
+  __device__ __forceinline__ int nt(const Grid& g) const { return gm == full ? r >> g.group : r / gm; }
+  __device__ __forceinline__ int mt(const Grid& g) const { return first + (gm == full ? r & (full - 1) : r % gm); }
 };
 
 template <int W>
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int run = 0, mine = 0;
   if constexpr (MODE == SPLIT) {
     const Walk w(g, unit);
-    const int mv = min(BT, a.M - w.mt() * BT);
+    const int mv = min(BT, a.M - w.mt(g) * BT);
     run = (mv + g.split - 1) / g.split;
     mine = max(0, min(run, mv - int(rank) * run));
     if (tid == 0 && mine) mbar_arrive_expect_tx(red_full, uint32_t(g.split - 1) * mine * kChannels * 4);
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (g.early_w) {
     const Walk w(g, unit);
     if (warp == 0 && w.more(g)) {
-      const int nt = w.nt();
+      const int nt = w.nt(g);
       uint32_t lead = 0;
       if constexpr (MODE == PAIR) lead = map_peer(full, 0);
       early = min(STAGES, kb1 - kb0);
@@ -213,8 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int kc = 0, s = 0;
     uint32_t phase = 1;  // of the ring's last round; its first finds every stage empty
     for (Walk w(g, unit); w.more(g) && ok; w.step(g, units)) {
-      const int wy = (w.nt() * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels;
-      const int ty = w.mt() * BT + (MODE == PAIR ? int(rank) * (BT / 2) : 0);
+      const int wy = (w.nt(g) * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels;
+      const int ty = w.mt(g) * BT + (MODE == PAIR ? int(rank) * (BT / 2) : 0);
       for (int kb = kb0; kb < kb1; ++kb, ++kc) {
         if (kc >= STAGES && !(ok = mbar_wait_warp(&empty[s], phase, a.err, DEV_ERR_TIMEOUT_PRODUCER))) break;
         uint8_t* st = ring + s * S::STAGE;
@@ -297,8 +300,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int n_next = 0, m_next = 0;
     Walk w(g, unit);
     auto fetch = [&] {
-      n_next = (w.nt() * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + ch;
-      m_next = w.mt() * BT;
+      n_next = (w.nt(g) * CG + (MODE == PAIR ? int(rank) : 0)) * kChannels + ch;
+      m_next = w.mt(g) * BT;
       ws_next = n_next < a.N ? a.w_scale[n_next] : 0.0f;
       bias_next = n_next < a.N && a.bias ? a.bias[n_next] : 0.0f;
 #pragma unroll
@@ -326,6 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok) ok = mbar_wait(&acc_full[b], u & 1, a.err, DEV_ERR_TIMEOUT_EPILOGUE);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
+      // the four warps of a quarter write their channels of a token together: whole stretches of the output's rows
+      // reach L2 and memory close in time (13,944 x 10,515 float, K = 128: 231 us apart, 167 together)
+      named_bar(2 + part4, 128);
       // before the columns from c on: the scales of their 32 tokens
       auto scales = [&](int c) {
         if (((c - c0) & 31) == 0) {
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < QW; ++j) part[(c0 + j) * kChannels + ch] = int(r[j]);
         }
         fence_proxy_async();
-        named_bar(2, 32 * kEpi);
+        named_bar(6, 32 * kEpi);
         if (ok && et < g.split && et != int(rank)) {
           const int count = max(0, min(run, mv - et * run));
           if (count)
@@ -515,6 +521,15 @@ __global__ void __launch_bounds__(256) k_lay_rows(const int8_t* src, size_t ld, 
   }
 }
 
+// Whether TMA can store to the output.
+bool can_box(const ProductArgs& a) {
+  return (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo * float_type_bytes(a.out_type) % 16 == 0;
+}
+
+// Token tiles walked together. One after the other the CTAs at work write neighbouring stretches of the same
+// rows, which is what counts while the weights stay in L2; eight tiles share each read of weights that do not.
+int walk_group(const ProductArgs& a) { return size_t(a.N) * a.K <= (size_t(24) << 20) ? 0 : 3; }
+
 template <int BT, int MODE, class T>
 cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtensorMap& map_t, int split, int early_w,
                    cudaStream_t st) {
@@ -534,10 +549,10 @@ cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtenso
   g.tiles_m = (a.M + BT - 1) / BT;
   g.split = split;
   g.early_w = early_w;
+  g.group = walk_group(a);
   CUtensorMap map_o = map_t;  // unused unless boxes
-  const size_t pitch = a.ldo * sizeof(T);
-  g.boxes = S::BOXES && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && pitch % 16 == 0;
-  if (g.boxes && make_tmap_store(&map_o, a.out, size_t(a.M), size_t(a.N), pitch, int(sizeof(T)), kBoxTokens<T, BT>))
+  g.boxes = S::BOXES && can_box(a);
+  if (g.boxes && make_tmap_store(&map_o, a.out, size_t(a.M), size_t(a.N), a.ldo * sizeof(T), int(sizeof(T)), kBoxTokens<T, BT>))
     return cudaErrorInvalidValue;
   const long long tiles = (long long)g.tiles_n * g.tiles_m;
   if (tiles > 0x7fffffffll / 16) return cudaErrorInvalidValue;
@@ -563,24 +578,60 @@ struct Pick {
   int bt, mode, split;
 };
 
-// The tile by an estimate of the slowest SM's cycles: the blocks of one tile, each the slower of its MMAs
-// (8,192 products a cycle) and its bytes (about 56 a cycle from L2), times the tiles an SM takes in turn, and
-// the last tile's epilogue. A split adds about 1,000 cycles of exchange.
-Pick pick(int M, int N, int K) {
+// How many clusters of `split` CTAs run at once (a cluster lies within a GPC, so not always SMs / split).
+int room_for(int split) {
+  static int known[kMaxDevices][kMaxSplit + 1] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int& n = known[dev][split];
+  if (!n) {
+    auto kernel = k_product_i8<16, SPLIT, float>;
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<16, SPLIT>::TOTAL);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(split * 64));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<16, SPLIT>::TOTAL;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int found = 0;
+    if (cudaOccupancyMaxActiveClusters(&found, kernel, &cfg) != cudaSuccess || found < 1) found = 1;
+    n = found;
+  }
+  return n;
+}
+
+// The tile by an estimate of the device time in cycles, whose parts are fits of measurements over 22 shapes (it
+// picks the fastest or within 5 % of it in all of them):
+//   block   128 bytes of depth of one tile: its MMAs (8,192 products a cycle); 145 cycles and its bytes at 125 a
+//           cycle for a CTA alone; its share of the 62 bytes a cycle and SM that L2 gives when all SMs read
+//   tile    `blocks` of them, or its epilogue where that takes longer: 400 cycles and 15 a token of 16-bit results, 22
+//           of float, 25 where TMA cannot store to the output
+//   turns   tiles that an SM takes one after the other; the last one's epilogue (or depth) is not hidden
+// A split's exchange adds 1,600 cycles and 60 a token, a pair 400.
+Pick pick(int M, int N, int K, bool boxes, bool wide) {
   const int sms = num_sms();
   const int KB = (K + kBlock - 1) / kBlock;
   Pick best{0, 0, 0};
-  double least = 1e300;
+  const float box_cost = wide ? 22.0f : 15.0f;
+  float least = 1e30f;
   auto consider = [&](int bt, int mode, int split) {
     const int cg = mode == PAIR ? 2 : 1;
-    const long long tiles = (long long)((N + 128 * cg - 1) / (128 * cg)) * ((M + bt - 1) / bt);
-    if (mode == SPLIT && tiles * split > sms) return;
+    const unsigned long long tiles = (unsigned long long)((N + 128 * cg - 1) / (128 * cg)) * ((M + bt - 1) / bt);
+    if (mode == SPLIT && tiles > (unsigned)room_for(split)) return;
     const int room = sms / cg;
-    const double turns = mode == SPLIT ? 1.0 : double((tiles + room - 1) / room);
-    const double block = std::max(2.0 * bt, std::max(64.0, (16384.0 + 128.0 * bt / cg) / 56.0));
-    const double main = ((KB + split - 1) / split) * block;
-    const double epi = 300.0 + 8.0 * std::min(bt, M);
-    const double t = turns * std::max(main, epi) + std::min(main, epi) + (mode == SPLIT ? 1000.0 : 0.0);
+    const float turns = float((tiles + room - 1) / room);
+    const float busy = std::min(1.0f, float(tiles) * cg * split / sms);
+    const float bytes = 16384.0f + 128.0f * bt / cg;
+    const float block = std::max({2.0f * bt, 145.0f + bytes / 125.0f, busy * bytes / 62.0f});
+    const float main = float((KB + split - 1) / split) * block;
+    const int tokens = std::min(bt, M);
+    const float epi = 400.0f + (boxes && mode != SPLIT && bt >= 64 ? box_cost : 25.0f) * tokens / split;
+    const float more = mode == SPLIT ? 1600.0f + 60.0f * tokens : mode == PAIR ? 400.0f : 0.0f;
+    const float t = turns * std::max(main, epi) + std::min(main, epi) + more;
     if (t < least) {
       least = t;
       best = {bt, mode, split};
@@ -590,7 +641,7 @@ Pick pick(int M, int N, int K) {
     consider(bt, ONE, 1);
     if (bt >= 128) consider(bt, PAIR, 1);
     if (bt <= 64)
-      for (int s : {2, 3, 4, 6, 8})
+      for (int s : {2, 3, 4, 8})
         if (s <= KB) consider(bt, SPLIT, s);
   }
   return best;
@@ -650,7 +701,7 @@ int launch_product_i8(const ProductArgs& args, uint8_t* scratch, int tokens_ahea
     return true;
   };
   if (!lay(a.a, a.lda, a.M) || !lay(a.w, a.ldw, a.N)) return -2;
-  const Pick p = pick(a.M, a.N, a.K);
+  const Pick p = pick(a.M, a.N, a.K, can_box(a), a.out_type == FT_F32);
   CUtensorMap map_w, map_t;
   if (make_tmap_i8_rows(&map_w, a.w, size_t(a.N), size_t(a.K), a.ldw, kChannels) ||
       make_tmap_i8_rows(&map_t, a.a, size_t(a.M), size_t(a.K), a.lda, p.mode == PAIR ? p.bt / 2 : p.bt))

@@ -1798,6 +1798,10 @@ int ae_linear_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, int x_type, cons
   q.x_type = x_type;
   q.inv_smooth = d_inv_smooth;
   q.ldq = align_up(K, 16);
+  if (const int r = launch_product_fused(a, q, c->stream); r <= 0) {
+    ++c->launches;
+    return r == 0 ? 0 : fail(c, AE_ERR_CUDA, "int8 product launch failed: code %d", r);
+  }
   uint8_t* scratch = nullptr;
   const size_t q_bytes = align_up(q.ldq * M, 256), s_bytes = align_up(size_t(M) * sizeof(float), 256);
   a.lda = q.ldq;

@@ -6,12 +6,9 @@
 #include "floatio.cuh"
 #include "kernels.h"
 #include "ptx.cuh"
-#include "rowmath.cuh"
+#include "rowquant.cuh"
 
 namespace ae {
-
-// Smallest row maximum that quantizes to anything but zeros: below it 127 / top would not be finite.
-constexpr float kTinyTop = 0x1p-119f;
 
 // ------------------------------------------------------------------------------- row quantization
 // TPR threads to a row. The row is read once into registers (NV 16-byte pieces a thread), or, when it is
@@ -75,20 +72,13 @@ __global__ void __launch_bounds__(TPR < 128 ? 128 : TPR) k_quant_rows(QuantArgs 
     for (int w = 0; w < TPR / 32; ++w) top = max(top, s_top[w]);
   }
   if (!live) return;
-  // a row that holds an infinity or a NaN has no scale: its scale is NaN, and so is its row of the product
-  const bool finite = top < 0x7f800000u;
-  const float m = __uint_as_float(top);
-  const bool any = finite && m >= kTinyTop;
-  const float inv = any ? 127.0f / m : 0.0f;
-  if (t == 0) a.scale[row] = finite ? (any ? m / 127.0f : 0.0f) : __uint_as_float(0x7fc00000u);
+  const RowScale rs(top);
+  if (t == 0) a.scale[row] = rs.scale;
   int8_t* q = a.q + size_t(row) * a.ldq;
   auto store = [&](int p, const float (&v)[VE]) {
     uint32_t w[VE / 4];
 #pragma unroll
-    for (int j = 0; j < VE / 4; ++j)
-      w[j] = !any ? 0u
-                  : pack_i8x4(quant_bits_scaled(v[4 * j] * inv), quant_bits_scaled(v[4 * j + 1] * inv),
-                              quant_bits_scaled(v[4 * j + 2] * inv), quant_bits_scaled(v[4 * j + 3] * inv));
+    for (int j = 0; j < VE / 4; ++j) w[j] = rs.four(v + 4 * j);
     if constexpr (VE == 8)
       *reinterpret_cast<uint2*>(q + p * VE) = make_uint2(w[0], w[1]);
     else

@@ -46,6 +46,9 @@ size_t product_scratch(const ProductArgs& a);
 // that one (whatever wrote the weights) is done once the product starts. *kernels += the launches made.
 int launch_product_i8(const ProductArgs& a, uint8_t* scratch, int tokens_ahead, cudaStream_t st, int* kernels);
 
+// The product from float activations in one kernel; 1 where it is not for these sizes (nothing is launched then).
+int launch_product_fused(const ProductArgs& a, const QuantArgs& q, cudaStream_t st);
+
 struct QkArgs {
   int tokens, heads[2], dim, rotary;  // heads[0] queries, heads[1] keys
   int type;

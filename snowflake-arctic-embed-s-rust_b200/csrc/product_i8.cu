@@ -27,6 +27,7 @@
 #include "linear_i8.h"
 #include "ptx.cuh"
 #include "rowmath.cuh"
+#include "rowquant.cuh"
 
 namespace ae {
 
@@ -46,16 +47,21 @@ constexpr int kBoxTokens = sizeof(T) == 4 || BT == 64 ? 16 : 32;
 
 enum Mode { ONE = 0, PAIR = 1, SPLIT = 2 };
 
-template <int BT, int MODE>
+// FUSE: the most depth blocks of quantized tokens a CTA holds (16 tokens, 2 KB a block).
+constexpr int kFuseBlocks = 32;
+constexpr size_t kFuseMost = 16 << 10;         // bytes of activations
+
+template <int BT, int MODE, bool FUSE = false>
 struct Shape {
   static constexpr int CG = MODE == PAIR ? 2 : 1;
   static constexpr int W_BYTES = kChannels * kBlock;
-  static constexpr int T_BYTES = BT / CG * kBlock;
+  static constexpr int T_BYTES = FUSE ? 0 : BT / CG * kBlock;           // tokens of a ring stage
+  static constexpr int TOK = FUSE ? kFuseBlocks * BT * kBlock : 0;          // all of a fused CTA's
   static constexpr int STAGE = W_BYTES + T_BYTES;
   static constexpr int RED = MODE == SPLIT ? (BT + kMaxSplit) * kChannels * 4 : 0;  // partial sums sent here
   static constexpr bool BOXES = MODE != SPLIT && BT >= 64;    // results leave as boxes where the output allows
   static constexpr int OUT = BOXES ? kEpi * kBoxBytes : 0;
-  static constexpr int FIXED = OUT + RED + kEpi * 32 * 4 + 256;
+  static constexpr int FIXED = OUT + RED + TOK + kEpi * 32 * 4 + (FUSE ? 128 : 0) + 256;
   static constexpr int FIT = (kSmemMost - FIXED) / STAGE;
   static constexpr int STAGES = FIT < 12 ? FIT : 12;
   static constexpr int TOTAL = FIXED + STAGES * STAGE;
@@ -64,6 +70,7 @@ struct Shape {
 };
 
 struct Grid {
+  QuantArgs q;   // FUSE: the float activations (q.q and q.scale unused)
   int tiles_n, tiles_m;
   int split;     // CTAs that share a tile's depth
   int early_w;   // the weights may be read before the kernel ahead has ended
@@ -107,24 +114,60 @@ __device__ __forceinline__ void tmem_ld_cols(uint32_t at, uint32_t (&r)[W]) {
 template <class T>
 __device__ __forceinline__ void put(T* p, float v) { *p = from_f32<T>(v); }
 
-template <int BT, int MODE, class T>
+// Eight activations of a row from k on, smoothed; zeros past the row's end.
+__device__ __forceinline__ void load8(const QuantArgs& q, const void* row, int k, bool wide, float (&v)[8]) {
+  if (wide && k + 8 <= q.K) {
+    if (q.x_type == FT_F32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(row) + k);
+      const float4 a = p[0], b = p[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      const uint4 p = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + k);
+      if (q.x_type == FT_F16) widen<__half>(p, v);
+      else widen<__nv_bfloat16>(p, v);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = 0.0f;
+      if (k + e < q.K) {
+        if (q.x_type == FT_F32) x = static_cast<const float*>(row)[k + e];
+        else if (q.x_type == FT_F16) x = to_f32(static_cast<const __half*>(row)[k + e]);
+        else x = to_f32(static_cast<const __nv_bfloat16*>(row)[k + e]);
+      }
+      v[e] = x;
+    }
+  }
+  if (q.inv_smooth) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (k + e < q.K) v[e] *= q.inv_smooth[k + e];
+  }
+}
+
+template <int BT, int MODE, class T, bool FUSE = false>
 __global__ void __launch_bounds__(kThreads, 1)
     k_product_i8(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_t,
                  const __grid_constant__ CUtensorMap map_o, ProductArgs a, Grid g) {
-  using S = Shape<BT, MODE>;
+  using S = Shape<BT, MODE, FUSE>;
   constexpr int STAGES = S::STAGES;
   constexpr int CG = S::CG;
+  static_assert(!FUSE || (BT == 16 && MODE != PAIR), "fused quantization is for up to 16 tokens");
   extern __shared__ __align__(1024) uint8_t smem_product[];  // the swizzles' 8-row atoms
   uint8_t* ring = smem_product;
-  uint8_t* s_out = ring + STAGES * S::STAGE;
+  uint8_t* s_tok = ring + STAGES * S::STAGE;
+  uint8_t* s_out = s_tok + S::TOK;
   int* red = reinterpret_cast<int*>(s_out + S::OUT);
   float* s_scale = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(red) + S::RED);  // 32 tokens' to a warp
-  uint64_t* full = reinterpret_cast<uint64_t*>(s_scale + kEpi * 32);
+  float* s_tscale = s_scale + kEpi * 32;            // FUSE: the tokens' scales, and the warps' maxima
+  uint32_t* s_top = reinterpret_cast<uint32_t*>(s_tscale + 16);
+  uint64_t* full = reinterpret_cast<uint64_t*>(s_tscale + (FUSE ? 32 : 0));
   uint64_t* empty = full + STAGES;
   uint64_t* acc_full = empty + STAGES;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* red_full = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_full + 1);
+  uint64_t* tok_full = red_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tok_full + 1);
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // uniform, for the compiler too
@@ -147,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&acc_empty[b], kEpi * CG);
     }
     mbar_init(red_full, 1);
+    mbar_init(tok_full, kEpi * 32);
     fence_mbar_init();
   }
   // SPLIT: the tile's tokens are finished in runs of `run`, CTA r taking `mine` of them from token r * run on
@@ -233,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               mbar_arrive_expect_tx(&full[s], S::STAGE);
               tma_load_2d(st, &map_w, &full[s], kb * kBlock, wy);
             }
-            tma_load_2d(st + S::W_BYTES, &map_t, &full[s], kb * kBlock, ty);
+            if constexpr (!FUSE) tma_load_2d(st + S::W_BYTES, &map_t, &full[s], kb * kBlock, ty);
           }
         }
         __syncwarp();
@@ -252,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int it = 0, s = 0;
       uint32_t phase = 0;
+      if constexpr (FUSE) ok = mbar_wait_warp(tok_full, 0, a.err, DEV_ERR_TIMEOUT_MMA);
       for (Walk w(g, unit); w.more(g) && ok; w.step(g, units), ++it) {
         const int b = it & 1, u = it >> 1;
         if (u >= 1 && !(ok = mbar_wait_warp(&acc_empty[b], (u - 1) & 1, a.err, DEV_ERR_TIMEOUT_MMA))) break;
@@ -261,7 +306,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(ok = mbar_wait_warp(&full[s], phase, a.err, DEV_ERR_TIMEOUT_MMA))) break;
           tc_fence_after();
           const uint64_t wd = sdesc_sw128(smem_u32(ring) + uint32_t(s) * S::STAGE);
-          const uint64_t td = wd + (S::W_BYTES >> 4);
+          const uint64_t td =
+              FUSE ? sdesc_sw128(smem_u32(s_tok) + uint32_t(kb - kb0) * (BT * kBlock)) : wd + (S::W_BYTES >> 4);
           if (elect_one()) {
 #pragma unroll
             for (int ks = 0; ks < kBlock / 32; ++ks) {  // 32 bytes on: + 2 in the descriptors' address field
@@ -307,11 +353,46 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int i = 0; i < TW; ++i) {
         const int t = lane + 32 * i, m = m_next + c0 + t;
-        as_next[i] = t < QW && m < a.M ? a.a_scale[m] : 0.0f;
+        if constexpr (!FUSE) as_next[i] = t < QW && m < a.M ? a.a_scale[m] : 0.0f;
       }
     };
     bool more = w.more(g);
     if (more) fetch();
+    if constexpr (FUSE) {
+      // The tokens of this CTA's depth, quantized here: every CTA takes the maxima over whole rows (the tokens
+      // are few, and L2 holds them) while its weights are on their way. `per` threads to a row.
+      const int per = (32 * kEpi) >> (a.M <= 1 ? 0 : 32 - __clz(a.M - 1));
+      const int row = et / per, t = et % per;
+      const bool mine_too = row < a.M;
+      const size_t size = g.q.x_type == FT_F32 ? 4 : 2;
+      const uint8_t* x = static_cast<const uint8_t*>(g.q.x) + (mine_too ? size_t(row) * g.q.ldx * size : 0);
+      const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+      uint32_t top = 0;
+      if (mine_too)
+        for (int p = t; p * 8 < a.K; p += per) {
+          float v[8];
+          load8(g.q, x, p * 8, wide, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
+        }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) s_top[warp - 2] = top;
+      named_bar(6, 32 * kEpi);
+      for (int i = 0; i < per / 32; ++i) top = max(top, s_top[et / per * (per / 32) + i]);
+      const RowScale rs(top);
+      if (mine_too && t == 0) s_tscale[row] = rs.scale;
+      if (mine_too)
+        for (int p = t; p < (kb1 - kb0) * (kBlock / 8); p += per) {
+          float v[8];
+          load8(g.q, x, kb0 * kBlock + p * 8, wide, v);
+          // 128-byte swizzle: 16-byte piece c of token r lies at c ^ (r % 8)
+          uint8_t* at = s_tok + (p >> 4) * (BT * kBlock) + row * kBlock + ((((p >> 1) & 7) ^ (row & 7)) << 4) + (p & 1) * 8;
+          *reinterpret_cast<uint2*>(at) = make_uint2(rs.four(v), rs.four(v + 4));
+        }
+      fence_proxy_async();
+      mbar_arrive(tok_full);
+      named_bar(6, 32 * kEpi);
+    }
     bool ok = true;
     int it = 0;
     for (; more; ++it) {
@@ -322,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float ws = ws_next, bias = bias_next;
       float as_own[TW];
 #pragma unroll
-      for (int i = 0; i < TW; ++i) as_own[i] = as_next[i];
+      for (int i = 0; i < TW; ++i) as_own[i] = FUSE ? s_tscale[(c0 + lane) & 15] : as_next[i];
       w.step(g, units);
       more = w.more(g);
       if (more) fetch();
@@ -480,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               int sum = part[c * kChannels + ch];
               for (int r = 0; r < g.split; ++r)
                 if (r != int(rank)) sum += red[(r * run + t) * kChannels + ch];
-              put(out + size_t(c) * a.ldo, fmaf(float(sum), a.a_scale[m0 + c] * ws, bias));
+              put(out + size_t(c) * a.ldo, fmaf(float(sum), (FUSE ? s_tscale[c] : a.a_scale[m0 + c]) * ws, bias));
             }
           }
         }
@@ -530,11 +611,11 @@ bool can_box(const ProductArgs& a) {
 // rows, which is what counts while the weights stay in L2; eight tiles share each read of weights that do not.
 int walk_group(const ProductArgs& a) { return size_t(a.N) * a.K <= (size_t(24) << 20) ? 0 : 3; }
 
-template <int BT, int MODE, class T>
+template <int BT, int MODE, class T, bool FUSE = false>
 cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtensorMap& map_t, int split, int early_w,
-                   cudaStream_t st) {
-  using S = Shape<BT, MODE>;
-  auto kernel = k_product_i8<BT, MODE, T>;
+                   cudaStream_t st, const QuantArgs* q = nullptr) {
+  using S = Shape<BT, MODE, FUSE>;
+  auto kernel = k_product_i8<BT, MODE, T, FUSE>;
   static bool ready[kMaxDevices] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -544,6 +625,7 @@ cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtenso
     ready[dev] = true;
   }
   Grid g{};
+  if (FUSE) g.q = *q;
   const int wide = kChannels * S::CG;
   g.tiles_n = (a.N + wide - 1) / wide;
   g.tiles_m = (a.M + BT - 1) / BT;
@@ -665,6 +747,12 @@ cudaError_t launch_pick(const Pick& p, const ProductArgs& a, const CUtensorMap& 
   return cudaErrorInvalidValue;
 }
 
+template <class T>
+cudaError_t launch_fused(const Pick& p, const ProductArgs& a, const CUtensorMap& w, const QuantArgs& q, cudaStream_t st) {
+  return p.mode == SPLIT ? launch<16, SPLIT, T, true>(a, w, w, p.split, 0, st, &q)
+                         : launch<16, ONE, T, true>(a, w, w, 1, 0, st, &q);
+}
+
 size_t row_pitch(int K) { return (size_t(K) + 15) / 16 * 16; }
 
 bool in_place(const int8_t* p, size_t ld, int rows) {
@@ -678,6 +766,23 @@ size_t product_scratch(const ProductArgs& a) {
   if (!in_place(a.a, a.lda, a.M)) n += (size_t(a.M) * row_pitch(a.K) + 255) / 256 * 256;
   if (!in_place(a.w, a.ldw, a.N)) n += size_t(a.N) * row_pitch(a.K);
   return n;
+}
+
+// Up to 16 tokens whose depth (its share of a split) fits a CTA's token blocks, and little enough to read in each of
+// some 130 CTAs at once. On the device one 4,096-deep bfloat16 token takes 6.7 us this way and 6.7 us in two kernels,
+// two 7.0 and 6.8, sixteen 11.8 and 7.0; a launch less spares the host about 2 us.
+int launch_product_fused(const ProductArgs& args, const QuantArgs& q, cudaStream_t st) {
+  ProductArgs a = args;
+  if (a.M > 16 || size_t(a.M) * a.K * float_type_bytes(q.x_type) > kFuseMost || !in_place(a.w, a.ldw, a.N)) return 1;
+  const Pick p = pick(a.M, a.N, a.K, can_box(a), a.out_type == FT_F32);
+  if (p.bt != 16 || ((a.K + kBlock - 1) / kBlock + p.split - 1) / p.split > kFuseBlocks) return 1;
+  if (a.N == 1) a.ldw = row_pitch(a.K);
+  CUtensorMap map_w;
+  if (make_tmap_i8_rows(&map_w, a.w, size_t(a.N), size_t(a.K), a.ldw, kChannels)) return -3;
+  const cudaError_t e = a.out_type == FT_F32   ? launch_fused<float>(p, a, map_w, q, st)
+                        : a.out_type == FT_F16 ? launch_fused<__half>(p, a, map_w, q, st)
+                                               : launch_fused<__nv_bfloat16>(p, a, map_w, q, st);
+  return e == cudaSuccess ? 0 : -100 - int(e);
 }
 
 int launch_product_i8(const ProductArgs& args, uint8_t* scratch, int tokens_ahead, cudaStream_t st, int* kernels) {

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "floatio.cuh"
+#include "gemm_i8.h"
 #include "kernels.h"
 #include "linear_i8.h"
 #include "ptx.cuh"
@@ -16,15 +17,14 @@ namespace ae {
 
 constexpr int kQkMaxDim = 512;
 
-// Position of token t: given, or counted from the start of its sequence (cu[s] <= t < cu[s + 1]); -1 if
-// there is none inside the table.
-__device__ __forceinline__ int qk_position(const QkArgs& a, int t) {
+// Position of token t: given, or counted from the start of its sequence (cu[s] <= t < cu[s + 1], s among lo .. hi);
+// -1 if there is none inside the table.
+__device__ __forceinline__ int qk_position(const QkArgs& a, int t, int lo, int hi) {
   int p;
   if (a.positions) {
     p = a.positions[t];
   } else {
-    int lo = 0, hi = a.n_seqs;  // the last s with cu[s] <= t, among 0 .. n_seqs
-    while (lo < hi) {
+    while (lo < hi) {  // the last s with cu[s] <= t
       const int mid = (lo + hi + 1) >> 1;
       if (a.cu[mid] <= uint32_t(t)) lo = mid;
       else hi = mid - 1;
@@ -32,6 +32,21 @@ __device__ __forceinline__ int qk_position(const QkArgs& a, int t) {
     p = lo < a.n_seqs && a.cu[lo] <= uint32_t(t) ? t - int(a.cu[lo]) : -1;
   }
   return p >= 0 && p < a.table_rows ? p : -1;
+}
+
+// The last s among 0 .. n with cu[s] <= t (0 if there is none), by a converged warp: 32 entries a round, so two
+// rounds for a thousand sequences where halving takes ten loads one after the other.
+__device__ __forceinline__ int warp_search(const uint32_t* cu, int n, int t) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int step = (hi - lo + 31) >> 5;
+    const long long at = lo + (long long)(lane + 1) * step;
+    const unsigned below = __ballot_sync(0xffffffffu, at <= hi && cu[at <= hi ? at : hi] <= uint32_t(t));
+    lo += __popc(below) * step;
+    hi = min(hi, lo + step - 1);
+  }
+  return lo;
 }
 
 // Heads of any dim at any address, a warp to a (token, head): lane l takes the pairs l, l + 32, ... and the unrotated dims after them.
@@ -49,7 +64,7 @@ __global__ void __launch_bounds__(256) k_qk_norm_rope(QkArgs a) {
   if (w) h -= a.heads[0];
   const T* x = static_cast<const T*>(a.x[w]) + size_t(t) * a.x_ts[w] + size_t(h) * a.x_hs[w];
   T* y = static_cast<T*>(a.y[w]) + size_t(t) * a.y_ts[w] + size_t(h) * a.y_hs[w];
-  const int p = a.rotary ? qk_position(a, t) : 0;
+  const int p = a.rotary ? qk_position(a, t, 0, a.n_seqs) : 0;
   if (p < 0) {
     if (lane == 0) record_err(a.err, DEV_ERR_BAD_POSITION);
     return;
@@ -110,191 +125,220 @@ struct Piece {
     else if constexpr (WORDS == 2) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
-  __device__ __forceinline__ void get(float (&v)[VE]) const {
-    if constexpr (sizeof(T) == 4) {
+  __device__ __forceinline__ void get(float2 (&v)[(VE + 1) / 2]) const {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) v[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) {
-        const float2 f = unpack2<T>(w[i]);
-        v[2 * i] = f.x, v[2 * i + 1] = f.y;
-      }
+    for (int i = 0; i < (VE + 1) / 2; ++i) {
+      if constexpr (sizeof(T) == 2) v[i] = unpack2<T>(w[i]);
+      else if constexpr (VE == 1) v[i] = make_float2(__uint_as_float(w[0]), 0.0f);
+      else v[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
     }
   }
-  __device__ __forceinline__ void set(const float (&v)[VE]) {
-    if constexpr (sizeof(T) == 4) {
+  __device__ __forceinline__ void set(const float2 (&v)[(VE + 1) / 2]) {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) w[i] = __float_as_uint(v[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < (VE + 1) / 2; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        w[i] = pack2<T>(v[i].x, v[i].y);
+      } else {
+        w[i * (VE == 1 ? 1 : 2)] = __float_as_uint(v[i].x);
+        if constexpr (VE > 1) w[2 * i + 1] = __float_as_uint(v[i].y);
+      }
     }
   }
 };
 
-constexpr int kQkThreads = 256;
-constexpr int kQkHeads = 4;  // heads to a thread
+constexpr int kQkThreads = 128;
 
 struct QkGrid {
   int lanes_log2;   // lanes to a head: the power of two from dim / (2 VE)
-  int slots[2];     // groups of kQkHeads heads of a token
-  int tokens[2];    // tokens to a block
+  int slots[2];     // groups of HPT heads of a token; a group of lanes takes one
   int blocks_q;     // blocks of queries; those of the keys follow
 };
 
-// Heads whose halves are whole pieces. A thread holds the two pieces of a head that rotate against one another
-// (or, unrotated, two neighbouring ones), for kQkHeads heads of one token, so a token's table row and the norm
-// weights are loaded once for four heads, all of a thread's loads of heads are in flight together, and every
-// element is read and written by one thread (outputs may be the inputs).
-template <class T, int VE>
-__global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
-  __shared__ int s_pos[kQkThreads];
-  pdl_trigger();
-  pdl_wait();
-  const int w = int(blockIdx.x) >= g.blocks_q;
-  const int t0 = (int(blockIdx.x) - (w ? g.blocks_q : 0)) * g.tokens[w];
-  const int nt = min(g.tokens[w], a.tokens - t0);
-  const int tid = threadIdx.x;
-  if (tid < nt) {
-    const int p = a.rotary ? qk_position(a, t0 + tid) : 0;
-    s_pos[tid] = p;
-    if (p < 0) record_err(a.err, DEV_ERR_BAD_POSITION);
-  }
-  __syncthreads();
-  const int lanes = 1 << g.lanes_log2;
-  const int j = tid & (lanes - 1);
-  const int turning = a.rotary / (2 * VE);       // lanes whose pieces are rotated
-  const bool in = j * 2 * VE < a.dim;
-  const bool turns = j < turning;
-  int d0, d1;                                     // where the two pieces start
-  if (turns && !a.neighbours) d0 = j * VE, d1 = a.rotary / 2 + j * VE;
-  else d0 = j * 2 * VE, d1 = d0 + VE;
-  float w0[VE], w1[VE];
-  if (in && a.weight[w]) {
-    Piece<float, VE < 4 ? VE : 4> v;
-    constexpr int S = VE < 4 ? VE : 4;
-#pragma unroll
-    for (int i = 0; i < VE; i += S) {
-      float f[S];
-      v.load(a.weight[w] + d0 + i);
-      v.get(f);
-#pragma unroll
-      for (int e = 0; e < S; ++e) w0[i + e] = f[e];
-      v.load(a.weight[w] + d1 + i);
-      v.get(f);
-#pragma unroll
-      for (int e = 0; e < S; ++e) w1[i + e] = f[e];
-    }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+
+// VE floats from an address that is a multiple of min(VE, 4) of them, as pairs (VE = 1: the first of one pair).
+template <int VE>
+__device__ __forceinline__ void load_floats(const float* p, float2 (&v)[(VE + 1) / 2]) {
+  if constexpr (VE == 1) {
+    v[0] = make_float2(*p, 0.0f);
+  } else if constexpr (VE == 2) {
+    v[0] = *reinterpret_cast<const float2*>(p);
   } else {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) w0[i] = w1[i] = 1.0f;
-  }
-  const int H = a.heads[w], slots = g.slots[w], groups = kQkThreads >> g.lanes_log2;
-  const T* x = static_cast<const T*>(a.x[w]);
-  T* y = static_cast<T*>(a.y[w]);
-  const int items = nt * slots;
-  for (int base = 0; base < items; base += groups) {  // uniform: the shuffles below take whole warps
-    const int item = base + (tid >> g.lanes_log2);
-    const int tt = item < items ? item / slots : 0;
-    const int t = t0 + tt, p = s_pos[tt];
-    const bool live = item < items && in && p >= 0;
-    const int h0 = (item - tt * slots) * kQkHeads;
-    Piece<T, VE> p0[kQkHeads], p1[kQkHeads];
-#pragma unroll
-    for (int h = 0; h < kQkHeads; ++h) {
-      if (live && h0 + h < H) {
-        const T* at = x + size_t(t) * a.x_ts[w] + size_t(h0 + h) * a.x_hs[w];
-        p0[h].load(at + d0);
-        p1[h].load(at + d1);
-      } else {
-#pragma unroll
-        for (int i = 0; i < Piece<T, VE>::WORDS; ++i) p0[h].w[i] = p1[h].w[i] = 0;
-      }
-    }
-    float c[VE], s[VE];
-    if (live && turns) {
-      const float* row = a.table + size_t(p) * a.rotary + j * VE;
-      constexpr int S = VE < 4 ? VE : 4;
-      Piece<float, S> v;
-#pragma unroll
-      for (int i = 0; i < VE; i += S) {
-        float f[S];
-        v.load(row + i);
-        v.get(f);
-#pragma unroll
-        for (int e = 0; e < S; ++e) c[i + e] = f[e];
-        v.load(row + a.rotary / 2 + i);
-        v.get(f);
-#pragma unroll
-        for (int e = 0; e < S; ++e) s[i + e] = f[e];
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) c[i] = 1.0f, s[i] = 0.0f;
-    }
-#pragma unroll
-    for (int h = 0; h < kQkHeads; ++h) {
-      float u[VE], v[VE];
-      p0[h].get(u);
-      p1[h].get(v);
-      if (a.norm) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VE; ++i) sum = fmaf(u[i], u[i], fmaf(v[i], v[i], sum));
-        for (int o = lanes >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float r = 1.0f / sqrtf(sum / float(a.dim) + a.eps);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) u[i] = u[i] * r * w0[i], v[i] = v[i] * r * w1[i];
-      }
-      if (turns) {
-        if (!a.neighbours) {
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            const float e = u[i], f = v[i];
-            u[i] = e * c[i] - f * s[i];
-            v[i] = f * c[i] + e * s[i];
-          }
-        } else if constexpr (VE >= 2) {
-#pragma unroll
-          for (int i = 0; i < VE; i += 2) {
-            const float e = u[i], f = u[i + 1], k = v[i], l = v[i + 1];
-            u[i] = e * c[i / 2] - f * s[i / 2];
-            u[i + 1] = f * c[i / 2] + e * s[i / 2];
-            v[i] = k * c[VE / 2 + i / 2] - l * s[VE / 2 + i / 2];
-            v[i + 1] = l * c[VE / 2 + i / 2] + k * s[VE / 2 + i / 2];
-          }
-        } else {
-          const float e = u[0], f = v[0];  // one pair to a thread
-          u[0] = e * c[0] - f * s[0];
-          v[0] = f * c[0] + e * s[0];
-        }
-      }
-      if (live && h0 + h < H) {
-        T* at = y + size_t(t) * a.y_ts[w] + size_t(h0 + h) * a.y_hs[w];
-        p0[h].set(u);
-        p1[h].set(v);
-        p0[h].store(at + d0);
-        p1[h].store(at + d1);
-      }
+    for (int i = 0; i < VE; i += 4) {
+      const float4 f = *reinterpret_cast<const float4*>(p + i);
+      v[i / 2] = make_float2(f.x, f.y);
+      v[i / 2 + 1] = make_float2(f.z, f.w);
     }
   }
 }
 
-template <class T, int VE>
-static cudaError_t launch_pieces(const QkArgs& a, cudaStream_t st) {
+// Heads whose halves are whole pieces. A thread holds the two pieces of a head that rotate against one another
+// (or, with neighbouring pairs or no rotation, two pieces in a row) for HPT heads of one token, so that a token's
+// table row and the norm weights, multiplied together once, serve all of them, all of a thread's loads of heads
+// are in flight together, and every element is read and written by one thread (outputs may be the inputs):
+//   y_0 = (r x_0) (w_0 c) + (r x_1) (-w_1 s),   y_1 = (r x_1) (w_1 c) + (r x_0) (w_0 s),   r = 1 / rms
+// in packed float pairs, 5 instructions an element with its conversions. HPT is 4 where that leaves threads for
+// every SM, else 1: one token takes 2.2 us with one head to a thread and 4.3 with four.
+template <class T, int VE, int HPT>
+__global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
+  constexpr int P = (VE + 1) / 2;                 // float pairs to a piece
+  __shared__ int s_pos[kQkThreads], s_seq[2];
+  pdl_trigger();
+  pdl_wait();
+  const int w = int(blockIdx.x) >= g.blocks_q;
+  const int tid = threadIdx.x, slots = g.slots[w];
+  const int groups = kQkThreads >> g.lanes_log2, group = tid >> g.lanes_log2;
+  // the block's first group's token and slot, then this group's
+  const unsigned block = blockIdx.x - (w ? unsigned(g.blocks_q) : 0u);
+  const unsigned long long first = (unsigned long long)block * groups;
+  const int t0 = first >> 32 ? int(first / unsigned(slots)) : int(unsigned(first) / unsigned(slots));
+  const int s0 = int(first - (unsigned long long)t0 * slots);
+  const int tt = (s0 + group) / slots, t = t0 + tt;
+  const int h0 = (s0 + group - tt * slots) * HPT;
+  const bool counted = a.rotary && !a.positions;  // places in sequences are searched for once a token
+  if (counted) {
+    const int nt = min((s0 + groups - 1) / slots + 1, a.tokens - t0);
+    if (tid < 64) {  // the sequences of the block's first and last token, and between them those of the others
+      const int found = warp_search(a.cu, a.n_seqs, t0 + (tid < 32 ? 0 : nt - 1));
+      if ((tid & 31) == 0) s_seq[tid >> 5] = found;
+    }
+    __syncthreads();
+    if (tid < nt) s_pos[tid] = qk_position(a, t0 + tid, s_seq[0], s_seq[1]);
+    __syncthreads();
+  }
+  const int lanes = 1 << g.lanes_log2;
+  const int j = tid & (lanes - 1);
+  const bool in = j * 2 * VE < a.dim;
+  const bool turns = j * 2 * VE < a.rotary;
+  int d0, d1;                                     // where the two pieces start
+  if (turns && !a.neighbours) d0 = j * VE, d1 = a.rotary / 2 + j * VE;
+  else d0 = j * 2 * VE, d1 = d0 + VE;
+  const int H = a.heads[w];
+  const float scale = 1.0f / float(a.dim);
+  const bool work = t < a.tokens && in;
+  const T* x = static_cast<const T*>(a.x[w]) + size_t(t) * a.x_ts[w] + size_t(h0) * a.x_hs[w];
+  Piece<T, VE> p0[HPT], p1[HPT];
+#pragma unroll
+  for (int h = 0; h < HPT; ++h) {
+    if (work && h0 + h < H) {
+      p0[h].load(x + d0);
+      p1[h].load(x + d1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < Piece<T, VE>::WORDS; ++i) p0[h].w[i] = p1[h].w[i] = 0;
+    }
+    x += a.x_hs[w];
+  }
+  int p = 0;
+  if (counted) {
+    p = t < a.tokens ? s_pos[tt] : 0;
+  } else if (a.rotary && t < a.tokens) {
+    p = a.positions[t];
+    if (p < 0 || p >= a.table_rows) p = -1;
+  }
+  const bool live = work && p >= 0;
+  if (p < 0 && j == 0 && h0 == 0) record_err(a.err, DEV_ERR_BAD_POSITION);
+  // a0, b0: factors of a first piece's own values and of their partners; a1, b1 of the second piece's
+  float2 a0[P], b0[P], a1[P], b1[P];
+  if (live && a.weight[w]) {
+    load_floats<VE>(a.weight[w] + d0, a0);
+    load_floats<VE>(a.weight[w] + d1, a1);
+  } else {
+#pragma unroll
+    for (int i = 0; i < P; ++i) a0[i] = a1[i] = make_float2(1.0f, 1.0f);
+  }
+  if (live && turns) {
+    const float* row = a.table + size_t(p) * a.rotary + j * VE;
+    float2 c[P], s[P];
+    load_floats<VE>(row, c);
+    load_floats<VE>(row + a.rotary / 2, s);
+    if (!a.neighbours || VE == 1) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        b0[i] = mul2(a1[i], make_float2(-s[i].x, -s[i].y));
+        b1[i] = mul2(a0[i], s[i]);
+        a0[i] = mul2(a0[i], c[i]);
+        a1[i] = mul2(a1[i], c[i]);
+      }
+    } else {
+      // pair i of the first piece turns by angle i, of the second by angle VE / 2 + i
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        const float c0 = i & 1 ? c[i / 2].y : c[i / 2].x, s0 = i & 1 ? s[i / 2].y : s[i / 2].x;
+        const int k = VE / 2 + i;
+        const float c1 = k & 1 ? c[k / 2].y : c[k / 2].x, s1 = k & 1 ? s[k / 2].y : s[k / 2].x;
+        b0[i] = make_float2(-a0[i].y * s0, a0[i].x * s0);
+        b1[i] = make_float2(-a1[i].y * s1, a1[i].x * s1);
+        a0[i] = mul2(a0[i], make_float2(c0, c0));
+        a1[i] = mul2(a1[i], make_float2(c1, c1));
+      }
+    }
+  }
+  T* y = static_cast<T*>(a.y[w]) + size_t(t) * a.y_ts[w] + size_t(h0) * a.y_hs[w];
+#pragma unroll
+  for (int h = 0; h < HPT; ++h) {
+    float2 u[P], v[P];
+    p0[h].get(u);
+    p1[h].get(v);
+    if (a.norm) {
+      float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+      for (int i = 0; i < P; ++i) sum = fma2(u[i], u[i], fma2(v[i], v[i], sum));
+      float all = sum.x + sum.y;
+      for (int o = lanes >> 1; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      const float r = rsqrtf(all * scale + a.eps);
+#pragma unroll
+      for (int i = 0; i < P; ++i) u[i] = mul2(u[i], make_float2(r, r)), v[i] = mul2(v[i], make_float2(r, r));
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float2 e = u[i], f = v[i];
+      u[i] = mul2(e, a0[i]);
+      v[i] = mul2(f, a1[i]);
+      if (turns) {  // not by factors of zero: an infinity stays in its own pair
+        if (!a.neighbours || VE == 1) {
+          u[i] = fma2(f, b0[i], u[i]);
+          v[i] = fma2(e, b1[i], v[i]);
+        } else {
+          u[i] = fma2(make_float2(e.y, e.x), b0[i], u[i]);
+          v[i] = fma2(make_float2(f.y, f.x), b1[i], v[i]);
+        }
+      }
+    }
+    if (live && h0 + h < H) {
+      p0[h].set(u);
+      p1[h].set(v);
+      p0[h].store(y + d0);
+      p1[h].store(y + d1);
+    }
+    y += a.y_hs[w];
+  }
+}
+
+
+template <class T, int VE, int HPT>
+static cudaError_t launch_heads(const QkArgs& a, cudaStream_t st) {
   QkGrid g{};
   while ((1 << g.lanes_log2) * 2 * VE < a.dim) ++g.lanes_log2;
   const int groups = kQkThreads >> g.lanes_log2;
   long long blocks[2];
   for (int w = 0; w < 2; ++w) {
-    g.slots[w] = (a.heads[w] + kQkHeads - 1) / kQkHeads;
-    g.tokens[w] = g.slots[w] ? std::max(1, std::min(kQkThreads, groups / g.slots[w])) : 1;
-    blocks[w] = g.slots[w] ? (a.tokens + g.tokens[w] - 1) / g.tokens[w] : 0;
+    g.slots[w] = (a.heads[w] + HPT - 1) / HPT;
+    blocks[w] = ((long long)a.tokens * g.slots[w] + groups - 1) / groups;
   }
   if (blocks[0] + blocks[1] > 0x7fffffffll) return cudaErrorInvalidValue;
   g.blocks_q = int(blocks[0]);
-  return launch_pdl(k_qk_pieces<T, VE>, dim3(unsigned(blocks[0] + blocks[1])), dim3(kQkThreads), 0, st, a, g);
+  return launch_pdl(k_qk_pieces<T, VE, HPT>, dim3(unsigned(blocks[0] + blocks[1])), dim3(kQkThreads), 0, st, a, g);
+}
+
+template <class T, int VE>
+static cudaError_t launch_pieces(const QkArgs& a, cudaStream_t st) {
+  // four heads to a thread from 256 threads an SM on (777 tokens of 10 + 5 heads of 80, 210 threads an SM: 5.5 us with
+  // four, 3.7 with one; 690 of 32 + 2 heads of 96 in float, 500 threads: 5.2 and 6.3)
+  const long long threads = (long long)a.tokens * ((a.heads[0] + 3) / 4 + (a.heads[1] + 3) / 4) * (a.dim / (2 * VE));
+  return threads >= 256ll * num_sms() ? launch_heads<T, VE, 4>(a, st) : launch_heads<T, VE, 1>(a, st);
 }
 
 // Whether every piece of VE elements (and of a head's weights and table rows) is whole and on its own size.

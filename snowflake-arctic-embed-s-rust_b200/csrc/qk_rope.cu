@@ -146,7 +146,7 @@ struct Piece {
   }
 };
 
-constexpr int kQkThreads = 128;
+constexpr int kQkThreads = 64;
 
 struct QkGrid {
   int lanes_log2;   // lanes to a head: the power of two from dim / (2 VE)
@@ -170,6 +170,68 @@ __device__ __forceinline__ void load_floats(const float* p, float2 (&v)[(VE + 1)
       const float4 f = *reinterpret_cast<const float4*>(p + i);
       v[i / 2] = make_float2(f.x, f.y);
       v[i / 2 + 1] = make_float2(f.z, f.w);
+    }
+  }
+}
+
+// Factors of a first piece's own values (a0) and of their partners (b0), and of a second piece's (a1, b1): on entry
+// a0 and a1 hold the weights, c and s the angles'.
+template <int VE>
+__device__ __forceinline__ void turn_factors(bool neighbours, const float2* c, const float2* s, float2* a0, float2* b0,
+                                             float2* a1, float2* b1) {
+  constexpr int P = (VE + 1) / 2;
+  if (!neighbours || VE == 1) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      b0[i] = mul2(a1[i], make_float2(-s[i].x, -s[i].y));
+      b1[i] = mul2(a0[i], s[i]);
+      a0[i] = mul2(a0[i], c[i]);
+      a1[i] = mul2(a1[i], c[i]);
+    }
+  } else {
+    // pair i of the first piece turns by angle i, of the second by angle VE / 2 + i
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const float c0 = i & 1 ? c[i / 2].y : c[i / 2].x, s0 = i & 1 ? s[i / 2].y : s[i / 2].x;
+      const int k = VE / 2 + i;
+      const float c1 = k & 1 ? c[k / 2].y : c[k / 2].x, s1 = k & 1 ? s[k / 2].y : s[k / 2].x;
+      b0[i] = make_float2(-a0[i].y * s0, a0[i].x * s0);
+      b1[i] = make_float2(-a1[i].y * s1, a1[i].x * s1);
+      a0[i] = mul2(a0[i], make_float2(c0, c0));
+      a1[i] = mul2(a1[i], make_float2(c1, c1));
+    }
+  }
+}
+
+// One head's two pieces, normed and turned in place; every lane of its group takes part in the sum.
+template <int VE>
+__device__ __forceinline__ void norm_and_turn(const QkArgs& a, float scale, int lanes, bool turns, const float2* a0,
+                                              const float2* b0, const float2* a1, const float2* b1, float2* u,
+                                              float2* v) {
+  constexpr int P = (VE + 1) / 2;
+  if (a.norm) {
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < P; ++i) sum = fma2(u[i], u[i], fma2(v[i], v[i], sum));
+    float all = sum.x + sum.y;
+    for (int o = lanes >> 1; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    const float r = rsqrtf(all * scale + a.eps);
+#pragma unroll
+    for (int i = 0; i < P; ++i) u[i] = mul2(u[i], make_float2(r, r)), v[i] = mul2(v[i], make_float2(r, r));
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const float2 e = u[i], f = v[i];
+    u[i] = mul2(e, a0[i]);
+    v[i] = mul2(f, a1[i]);
+    if (turns) {  // not by factors of zero: an infinity stays in its own pair
+      if (!a.neighbours || VE == 1) {
+        u[i] = fma2(f, b0[i], u[i]);
+        v[i] = fma2(e, b1[i], v[i]);
+      } else {
+        u[i] = fma2(make_float2(e.y, e.x), b0[i], u[i]);
+        v[i] = fma2(make_float2(f.y, f.x), b1[i], v[i]);
+      }
     }
   }
 }
@@ -240,7 +302,6 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
   }
   const bool live = work && p >= 0;
   if (p < 0 && j == 0 && h0 == 0) record_err(a.err, DEV_ERR_BAD_POSITION);
-  // a0, b0: factors of a first piece's own values and of their partners; a1, b1 of the second piece's
   float2 a0[P], b0[P], a1[P], b1[P];
   if (live && a.weight[w]) {
     load_floats<VE>(a.weight[w] + d0, a0);
@@ -254,27 +315,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
     float2 c[P], s[P];
     load_floats<VE>(row, c);
     load_floats<VE>(row + a.rotary / 2, s);
-    if (!a.neighbours || VE == 1) {
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        b0[i] = mul2(a1[i], make_float2(-s[i].x, -s[i].y));
-        b1[i] = mul2(a0[i], s[i]);
-        a0[i] = mul2(a0[i], c[i]);
-        a1[i] = mul2(a1[i], c[i]);
-      }
-    } else {
-      // pair i of the first piece turns by angle i, of the second by angle VE / 2 + i
-#pragma unroll
-      for (int i = 0; i < P; ++i) {
-        const float c0 = i & 1 ? c[i / 2].y : c[i / 2].x, s0 = i & 1 ? s[i / 2].y : s[i / 2].x;
-        const int k = VE / 2 + i;
-        const float c1 = k & 1 ? c[k / 2].y : c[k / 2].x, s1 = k & 1 ? s[k / 2].y : s[k / 2].x;
-        b0[i] = make_float2(-a0[i].y * s0, a0[i].x * s0);
-        b1[i] = make_float2(-a1[i].y * s1, a1[i].x * s1);
-        a0[i] = mul2(a0[i], make_float2(c0, c0));
-        a1[i] = mul2(a1[i], make_float2(c1, c1));
-      }
-    }
+    turn_factors<VE>(a.neighbours, c, s, a0, b0, a1, b1);
   }
   T* y = static_cast<T*>(a.y[w]) + size_t(t) * a.y_ts[w] + size_t(h0) * a.y_hs[w];
 #pragma unroll
@@ -282,31 +323,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
     float2 u[P], v[P];
     p0[h].get(u);
     p1[h].get(v);
-    if (a.norm) {
-      float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-      for (int i = 0; i < P; ++i) sum = fma2(u[i], u[i], fma2(v[i], v[i], sum));
-      float all = sum.x + sum.y;
-      for (int o = lanes >> 1; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      const float r = rsqrtf(all * scale + a.eps);
-#pragma unroll
-      for (int i = 0; i < P; ++i) u[i] = mul2(u[i], make_float2(r, r)), v[i] = mul2(v[i], make_float2(r, r));
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const float2 e = u[i], f = v[i];
-      u[i] = mul2(e, a0[i]);
-      v[i] = mul2(f, a1[i]);
-      if (turns) {  // not by factors of zero: an infinity stays in its own pair
-        if (!a.neighbours || VE == 1) {
-          u[i] = fma2(f, b0[i], u[i]);
-          v[i] = fma2(e, b1[i], v[i]);
-        } else {
-          u[i] = fma2(make_float2(e.y, e.x), b0[i], u[i]);
-          v[i] = fma2(make_float2(f.y, f.x), b1[i], v[i]);
-        }
-      }
-    }
+    norm_and_turn<VE>(a, scale, lanes, turns, a0, b0, a1, b1, u, v);
     if (live && h0 + h < H) {
       p0[h].set(u);
       p1[h].set(v);

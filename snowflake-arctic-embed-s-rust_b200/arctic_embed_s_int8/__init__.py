@@ -14,7 +14,7 @@ import os
 import numpy as np
 
 from . import ae8
-from ._lib import AeError, LayerDesc, LinearDesc, ModelDesc, check, lib
+from ._lib import AeError, LayerDesc, LinearDesc, ModelDesc, check, lib, tensors
 
 HIDDEN_SIZE = 384
 MAX_POSITIONS = 512
@@ -51,71 +51,6 @@ def _ptr(a) -> int | None:
         assert a.flags["C_CONTIGUOUS"], "array must be C-contiguous"
         return a.ctypes.data
     return a.data_ptr()  # torch tensor (device memory)
-
-
-class _TensorTypes:
-    """torch's dtypes as the general operators take them, looked up once: a call's checks cost about as much as
-    its launch on small inputs."""
-
-    def __init__(self):
-        import torch
-
-        self.i8, self.i32, self.f32 = torch.int8, torch.int32, torch.float32
-        self.offsets = (torch.int32, torch.uint32)
-        self.floats = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # AE_F32 / AE_F16 / AE_BF16
-
-
-_tensor_types = None
-
-
-def _types() -> _TensorTypes:
-    global _tensor_types
-    if _tensor_types is None:
-        _tensor_types = _TensorTypes()
-    return _tensor_types
-
-
-def _refuse(t, what: str, shape: tuple, dtype, device: int):
-    if t.shape != shape:
-        raise ValueError(f"{what} must be {shape}, not {tuple(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{what} must be {dtype}, not {t.dtype}")
-    if t.get_device() != device:
-        raise ValueError(f"{what} must be in device memory of GPU {device}")
-    raise ValueError(f"{what} must be contiguous along its last axis")
-
-
-def _vector(t, what: str, n: int, dtype, device: int) -> int:
-    """Address of a contiguous [n] device tensor."""
-    if t.shape != (n,) or t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
-        _refuse(t, what, (n,), dtype, device)
-    return t.data_ptr()
-
-
-def _matrix(t, what: str, rows: int, cols: int, dtype, device: int) -> tuple[int, int]:
-    """Address and row pitch of a [rows, cols] device tensor whose rows are contiguous; the pitch of a single
-    row is the row's own length."""
-    pitch, step = t.stride()
-    if t.shape != (rows, cols) or t.dtype is not dtype or t.get_device() != device or (
-            step != 1 and cols > 1 and rows):
-        _refuse(t, what, (rows, cols), dtype, device)
-    return t.data_ptr(), pitch if rows > 1 and cols else cols
-
-
-def _heads(t, what: str, shape: tuple, dtype, device: int) -> tuple[int, int, int]:
-    """Address, token stride and head stride of a [tokens, heads, dim] device tensor with contiguous heads."""
-    token, head, step = t.stride()
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != device or (
-            step != 1 and shape[2] > 1 and t.numel()):
-        _refuse(t, what, shape, dtype, device)
-    return t.data_ptr(), token, head
-
-
-def _float_type(t, what: str) -> int:
-    code = _types().floats.get(t.dtype)
-    if code is None:
-        raise ValueError(f"{what} must be float32, float16 or bfloat16, not {t.dtype}")
-    return code
 
 
 def _linear_desc(lin: ae8.QuantizedLinear | None, keep: list) -> LinearDesc:
@@ -262,31 +197,14 @@ class Engine:
         """ae_matmul_i8: out[m, n] = (sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n]) + bias[n] on device
         tensors: a [M, K] and w [N, K] int8, a_scale [M], w_scale [N] and bias [N] float32, out [M, N]
         float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream."""
-        ty, dev = _types(), self.device
-        (M, K), N = a.shape, w.shape[0]
-        out_type = _float_type(out, "out")
-        ap, lda = _matrix(a, "a", M, K, ty.i8, dev)
-        wp, ldw = _matrix(w, "w", N, K, ty.i8, dev)
-        op, ldo = _matrix(out, "out", M, N, out.dtype, dev)
-        code = lib().ae_matmul_i8(self._h, M, N, K, ap, lda, _vector(a_scale, "a_scale", M, ty.f32, dev), wp, ldw,
-                                  _vector(w_scale, "w_scale", N, ty.f32, dev),
-                                  None if bias is None else _vector(bias, "bias", N, ty.f32, dev), out_type, op, ldo)
+        code = tensors().matmul_i8(self._h.value, self.device, a, a_scale, w, w_scale, out, bias)
         if code:
             self._check(code)
 
     def linear_i8(self, x, w, w_scale, out, bias=None, inv_smooth=None) -> None:
         """ae_linear_i8: the same product from float activations x [M, K] (float32, float16 or bfloat16),
         multiplied by inv_smooth [K] and quantized to int8 with a scale for each token on the way."""
-        ty, dev = _types(), self.device
-        (M, K), N = x.shape, w.shape[0]
-        x_type, out_type = _float_type(x, "x"), _float_type(out, "out")
-        xp, ldx = _matrix(x, "x", M, K, x.dtype, dev)
-        wp, ldw = _matrix(w, "w", N, K, ty.i8, dev)
-        op, ldo = _matrix(out, "out", M, N, out.dtype, dev)
-        code = lib().ae_linear_i8(self._h, M, N, K, x_type, xp, ldx,
-                                  None if inv_smooth is None else _vector(inv_smooth, "inv_smooth", K, ty.f32, dev),
-                                  wp, ldw, _vector(w_scale, "w_scale", N, ty.f32, dev),
-                                  None if bias is None else _vector(bias, "bias", N, ty.f32, dev), out_type, op, ldo)
+        code = tensors().linear_i8(self._h.value, self.device, x, inv_smooth, w, w_scale, out, bias)
         if code:
             self._check(code)
 
@@ -298,35 +216,9 @@ class Engine:
         k [T, k_heads, dim] and the rotation of their first table.shape[1] dims, into q_out and k_out (which
         may be q and k). table [rows, rotary] float32 is rope_table's; a token's position is positions[t]
         (int32), or its place in its sequence of cu (int32 or uint32 [n_seqs + 1])."""
-        ty, dev, dt = _types(), self.device, q.dtype
-        code = _float_type(q, "q")
-        T, Hq, D = shape = q.shape
-        Hk = k.shape[1]
-        k_shape = (T, Hk, D)
-        rows = rotary = n_seqs = 0
-        tp = pp = cp = None
-        if table is not None:
-            rows, rotary = table.shape
-            tp, pitch = _matrix(table, "table", rows, rotary, ty.f32, dev)
-            if pitch != rotary:
-                raise ValueError("table must be contiguous")
-            if positions is not None:
-                pp = _vector(positions, "positions", T, ty.i32, dev)
-            elif cu is not None:
-                n_seqs = cu.shape[0] - 1
-                if cu.dtype not in ty.offsets:
-                    raise ValueError(f"cu must be int32 or uint32, not {cu.dtype}")
-                cp = _vector(cu, "cu", n_seqs + 1, cu.dtype, dev)
-            else:
-                raise ValueError("a rotation needs positions or cu")
-        code = lib().ae_qk_norm_rope(
-            self._h, code, T, Hq, Hk, D, rotary,
-            (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM),
-            *_heads(q, "q", shape, dt, dev), *_heads(k, "k", k_shape, dt, dev),
-            *_heads(q_out, "q_out", shape, dt, dev), *_heads(k_out, "k_out", k_shape, dt, dev),
-            None if q_weight is None else _vector(q_weight, "q_weight", D, ty.f32, dev),
-            None if k_weight is None else _vector(k_weight, "k_weight", D, ty.f32, dev),
-            eps, tp, rows, pp, cp, n_seqs)
+        flags = (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM)
+        code = tensors().qk_norm_rope(self._h.value, self.device, q, k, q_out, k_out, table, positions, cu, q_weight,
+                                      k_weight, eps, flags)
         if code:
             self._check(code)
 

@@ -8,9 +8,11 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import sys
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libarctic_cuda.so")
+TENSORS_PATH = os.path.join(_PKG_ROOT, "lib", "arctic_tensors.so")
 CSRC = os.path.join(_PKG_ROOT, "csrc")
 HEADER = os.path.join(os.path.dirname(_PKG_ROOT), "include", "arctic_cuda.h")
 
@@ -68,11 +70,8 @@ class ModelDesc(C.Structure):
 
 
 def build(force: bool = False) -> str:
-    """Compiles the CUDA library for sm_100a (make in csrc/)."""
-    if force or not os.path.exists(LIB_PATH):
-        subprocess.run(["make", "-s", "-C", CSRC, "-j4"], check=True)
-    else:
-        subprocess.run(["make", "-s", "-C", CSRC, "-j4"], check=True)
+    """Compiles the CUDA library for sm_100a and the module of its calls on torch tensors (make in csrc/)."""
+    subprocess.run(["make", "-s", "-C", CSRC, "-j4", "python", f"PYTHON={sys.executable}"], check=True)
     return LIB_PATH
 
 
@@ -141,3 +140,24 @@ def check(ctx, code: int) -> None:
     if code != AE_OK:
         msg = lib().ae_last_error(ctx)
         raise AeError(code, msg.decode() if msg else "")
+
+
+_tensors = None
+
+
+def tensors():
+    """The module of the general operators' calls on torch tensors (csrc/tensors.cpp), bound to lib()."""
+    global _tensors
+    if _tensors is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries, which the module uses)
+
+        if not os.path.exists(TENSORS_PATH):
+            raise RuntimeError(f"{TENSORS_PATH} is missing: build it with `make -C {CSRC} python`")
+        spec = importlib.util.spec_from_file_location("arctic_tensors", TENSORS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.bind(*(C.cast(getattr(lib(), n), C.c_void_p).value for n in ("ae_matmul_i8", "ae_linear_i8", "ae_qk_norm_rope")))
+        _tensors = module
+    return _tensors

@@ -609,7 +609,7 @@ bool can_box(const ProductArgs& a) {
 
 // Token tiles walked together. One after the other the CTAs at work write neighbouring stretches of the same
 // rows, which is what counts while the weights stay in L2; eight tiles share each read of weights that do not.
-int walk_group(const ProductArgs& a) { return size_t(a.N) * a.K <= (size_t(24) << 20) ? 0 : 3; }
+int walk_group(const ProductArgs& a) { return size_t(a.N) * a.K <= (size_t(64) << 20) ? 0 : 3; }
 
 template <int BT, int MODE, class T, bool FUSE = false>
 cudaError_t launch(const ProductArgs& a, const CUtensorMap& map_w, const CUtensorMap& map_t, int split, int early_w,

@@ -524,10 +524,23 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld_cols<CW>(lane_base + uint32_t(b * BT + c), r);
             tmem_ld_wait();
             T* p = out + size_t(c) * a.ldo;
-            if (live) {
+            // Whole chunks in packed pairs (512 x 1,002, K = 384 to bfloat16: 3.0 -> 2.8 us), but not the wide tiles of
+            // long batches: there the four warps' stores of a token, value by value, still reach a row's shared
+            // sectors together (13,944 x 10,515, K = 128 to float: 121 us value by value, 154 in pairs)
+            if (CW <= 16 && live && c + CW <= c_end) {
+#pragma unroll
+              for (int j = 0; j < CW; j += 2) {
+                const float2 v = __ffma2_rn(make_float2(float(int(r[j])), float(int(r[j + 1]))),
+                                            __fmul2_rn(*reinterpret_cast<const float2*>(as + j), make_float2(ws, ws)),
+                                            make_float2(bias, bias));
+                put(p, v.x);
+                put(p + a.ldo, v.y);
+                p += 2 * a.ldo;
+              }
+            } else if (live) {
 #pragma unroll
               for (int j = 0; j < CW; ++j) {
-                if (c + j < mv) put(p, fmaf(float(int(r[j])), as[j] * ws, bias));
+                if (c + j < c_end) put(p, fmaf(float(int(r[j])), as[j] * ws, bias));
                 p += a.ldo;
               }
             }
@@ -691,7 +704,7 @@ int room_for(int split) {
 //   block   128 bytes of depth of one tile: its MMAs (8,192 products a cycle); 145 cycles and its bytes at 125 a
 //           cycle for a CTA alone; its share of the 62 bytes a cycle and SM that L2 gives when all SMs read
 //   tile    `blocks` of them, or its epilogue where that takes longer: 400 cycles and 15 a token of 16-bit results, 22
-//           of float, 25 where TMA cannot store to the output
+//           of float, 25 where TMA cannot store to the output, a tenth less in a pair
 //   turns   tiles that an SM takes one after the other; the last one's epilogue (or depth) is not hidden
 // A split's exchange adds 1,600 cycles and 60 a token, a pair 400.
 Pick pick(int M, int N, int K, bool boxes, bool wide) {
@@ -711,7 +724,8 @@ Pick pick(int M, int N, int K, bool boxes, bool wide) {
     const float block = std::max({2.0f * bt, 145.0f + bytes / 125.0f, busy * bytes / 62.0f});
     const float main = float((KB + split - 1) / split) * block;
     const int tokens = std::min(bt, M);
-    const float epi = 400.0f + (boxes && mode != SPLIT && bt >= 64 ? box_cost : 25.0f) * tokens / split;
+    const float epi = (mode == PAIR ? 0.9f : 1.0f) *
+                      (400.0f + (boxes && mode != SPLIT && bt >= 64 ? box_cost : 25.0f) * tokens / split);
     const float more = mode == SPLIT ? 1600.0f + 60.0f * tokens : mode == PAIR ? 400.0f : 0.0f;
     const float t = turns * std::max(main, epi) + std::min(main, epi) + more;
     if (t < least) {

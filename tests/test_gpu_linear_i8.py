@@ -268,6 +268,57 @@ def test_streams(eng):
         assert all(torch.equal(want[i], o) for o in outs[i])
 
 
+@pytest.mark.parametrize("M", [1, 64, 700])
+def test_operands_written_just_before(eng, M):
+    """Weights, activations and scales that the kernel ahead on the stream has just written, call after call with
+    nothing in between: each result is that of the operands as they stood."""
+    N, K, rounds = 512, 2048, 24
+    r = rng(M)
+    ws = torch.from_numpy(r.integers(-127, 128, (rounds, N, K), dtype=np.int8)).cuda()
+    xs = torch.from_numpy(r.normal(0, 1, (rounds, M, K)).astype(np.float32)).cuda()
+    w_s = torch.from_numpy(r.uniform(1e-4, 1e-3, (rounds, N)).astype(np.float32)).cuda()
+    want = torch.empty(rounds, M, N, device="cuda")
+    for i in range(rounds):
+        eng.linear_i8(xs[i], ws[i], w_s[i], want[i])
+        eng.sync()
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = torch.empty_like(want)
+    try:
+        eng.set_stream(s)
+        with torch.cuda.stream(s):
+            w, x, sc = torch.zeros_like(ws[0]), torch.zeros_like(xs[0]), torch.zeros_like(w_s[0])
+            for i in range(rounds):
+                x.copy_(xs[i])
+                sc.copy_(w_s[i])
+                w.copy_(ws[i])
+                eng.linear_i8(x, w, sc, got[i])
+        s.synchronize()
+    finally:
+        eng.set_stream(None)
+    eng.sync()
+    assert torch.equal(got, want)
+
+
+def test_calls_in_a_chain(eng):
+    """One call's result is the next one's input."""
+    M, D = 300, 1024
+    r = rng(8)
+    w = [torch.from_numpy(r.integers(-127, 128, (D, D), dtype=np.int8)).cuda() for _ in range(6)]
+    ws = torch.full((D,), 1.0 / (127 * 18), device="cuda")
+    x = torch.from_numpy(r.normal(0, 1, (M, D)).astype(np.float32)).cuda()
+    steps = [x]
+    for v in w:
+        steps.append(torch.empty(M, D, device="cuda"))
+        eng.linear_i8(steps[-2], v, ws, steps[-1])
+        eng.sync()
+    again = [torch.empty(M, D, device="cuda") for _ in w]
+    for i, v in enumerate(w):
+        eng.linear_i8(x if i == 0 else again[i - 1], v, ws, again[i])
+    eng.sync()
+    assert all(torch.equal(a, b) for a, b in zip(again, steps[1:]))
+
+
 def test_graph_capture(eng):
     """A captured call replays on new inputs."""
     M, N, K = 4, 1152, 384

@@ -20,6 +20,7 @@
 //   SPLIT  a cluster of 2..8 CTAs splits the depth of one tile and adds the partial sums through distributed
 //          shared memory, where there are too few tiles for the SMs.
 #include <algorithm>
+#include <cmath>
 
 #include "floatio.cuh"
 #include "gemm_i8.h"
@@ -722,11 +723,10 @@ Pick pick(int M, int N, int K, bool boxes, bool wide) {
   float least = 1e30f;
   auto consider = [&](int bt, int mode, int split) {
     const int cg = mode == PAIR ? 2 : 1;
-    const unsigned long long tiles = (unsigned long long)((N + 128 * cg - 1) / (128 * cg)) * ((M + bt - 1) / bt);
-    if (mode == SPLIT && tiles > (unsigned)room_for(split)) return;
-    const int room = sms / cg;
-    const float turns = float((tiles + room - 1) / room);
-    const float busy = std::min(1.0f, float(tiles) * cg * split / sms);
+    const float tiles = float((N + 128 * cg - 1) / (128 * cg)) * float((M + bt - 1) / bt);
+    if (mode == SPLIT && tiles > float(room_for(split))) return;
+    const float turns = std::ceil(tiles / float(sms / cg));
+    const float busy = std::min(1.0f, tiles * float(cg * split) / float(sms));
     const float bytes = 16384.0f + 128.0f * bt / cg;
     const float block = std::max({2.0f * bt, 145.0f + bytes / 125.0f, busy * bytes / 62.0f});
     const float main = float((KB + split - 1) / split) * block;

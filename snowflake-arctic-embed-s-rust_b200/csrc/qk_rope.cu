@@ -176,11 +176,11 @@ __device__ __forceinline__ void load_floats(const float* p, float2 (&v)[(VE + 1)
 
 // Factors of a first piece's own values (a0) and of their partners (b0), and of a second piece's (a1, b1): on entry
 // a0 and a1 hold the weights, c and s the angles'.
-template <int VE>
-__device__ __forceinline__ void turn_factors(bool neighbours, const float2* c, const float2* s, float2* a0, float2* b0,
+template <int VE, bool NEIGHBOURS>
+__device__ __forceinline__ void turn_factors(const float2* c, const float2* s, float2* a0, float2* b0,
                                              float2* a1, float2* b1) {
   constexpr int P = (VE + 1) / 2;
-  if (!neighbours || VE == 1) {
+  if constexpr (!NEIGHBOURS || VE == 1) {
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       b0[i] = mul2(a1[i], make_float2(-s[i].x, -s[i].y));
@@ -204,7 +204,7 @@ __device__ __forceinline__ void turn_factors(bool neighbours, const float2* c, c
 }
 
 // One head's two pieces, normed and turned in place; every lane of its group takes part in the sum.
-template <int VE>
+template <int VE, bool NEIGHBOURS>
 __device__ __forceinline__ void norm_and_turn(const QkArgs& a, float scale, int lanes, bool turns, const float2* a0,
                                               const float2* b0, const float2* a1, const float2* b1, float2* u,
                                               float2* v) {
@@ -225,7 +225,7 @@ __device__ __forceinline__ void norm_and_turn(const QkArgs& a, float scale, int 
     u[i] = mul2(e, a0[i]);
     v[i] = mul2(f, a1[i]);
     if (turns) {  // not by factors of zero: an infinity stays in its own pair
-      if (!a.neighbours || VE == 1) {
+      if constexpr (!NEIGHBOURS || VE == 1) {
         u[i] = fma2(f, b0[i], u[i]);
         v[i] = fma2(e, b1[i], v[i]);
       } else {
@@ -243,7 +243,7 @@ __device__ __forceinline__ void norm_and_turn(const QkArgs& a, float scale, int 
 //   y_0 = (r x_0) (w_0 c) + (r x_1) (-w_1 s),   y_1 = (r x_1) (w_1 c) + (r x_0) (w_0 s),   r = 1 / rms
 // in packed float pairs, 5 instructions an element with its conversions. HPT is 4 where that leaves threads for
 // every SM, else 1: one token takes 2.2 us with one head to a thread and 4.3 with four.
-template <class T, int VE, int HPT>
+template <class T, int VE, int HPT, bool NEIGHBOURS>
 __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
   constexpr int P = (VE + 1) / 2;                 // float pairs to a piece
   __shared__ int s_pos[kQkThreads], s_seq[2];
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
   const bool in = j * 2 * VE < a.dim;
   const bool turns = j * 2 * VE < a.rotary;
   int d0, d1;                                     // where the two pieces start
-  if (turns && !a.neighbours) d0 = j * VE, d1 = a.rotary / 2 + j * VE;
+  if (turns && !NEIGHBOURS) d0 = j * VE, d1 = a.rotary / 2 + j * VE;
   else d0 = j * 2 * VE, d1 = d0 + VE;
   const int H = a.heads[w];
   const float scale = 1.0f / float(a.dim);
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
     float2 c[P], s[P];
     load_floats<VE>(row, c);
     load_floats<VE>(row + a.rotary / 2, s);
-    turn_factors<VE>(a.neighbours, c, s, a0, b0, a1, b1);
+    turn_factors<VE, NEIGHBOURS>(c, s, a0, b0, a1, b1);
   }
   T* y = static_cast<T*>(a.y[w]) + size_t(t) * a.y_ts[w] + size_t(h0) * a.y_hs[w];
 #pragma unroll
@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kQkThreads) k_qk_pieces(QkArgs a, QkGrid g) {
     float2 u[P], v[P];
     p0[h].get(u);
     p1[h].get(v);
-    norm_and_turn<VE>(a, scale, lanes, turns, a0, b0, a1, b1, u, v);
+    norm_and_turn<VE, NEIGHBOURS>(a, scale, lanes, turns, a0, b0, a1, b1, u, v);
     if (live && h0 + h < H) {
       p0[h].set(u);
       p1[h].set(v);
@@ -347,7 +347,8 @@ static cudaError_t launch_heads(const QkArgs& a, cudaStream_t st) {
   }
   if (blocks[0] + blocks[1] > 0x7fffffffll) return cudaErrorInvalidValue;
   g.blocks_q = int(blocks[0]);
-  return launch_pdl(k_qk_pieces<T, VE, HPT>, dim3(unsigned(blocks[0] + blocks[1])), dim3(kQkThreads), 0, st, a, g);
+  return launch_pdl(a.neighbours ? k_qk_pieces<T, VE, HPT, true> : k_qk_pieces<T, VE, HPT, false>,
+                    dim3(unsigned(blocks[0] + blocks[1])), dim3(kQkThreads), 0, st, a, g);
 }
 
 template <class T, int VE>

@@ -86,10 +86,11 @@ __device__ __forceinline__ uint32_t row_top(float top, int turn) {
 // TPR threads to a row, which is read once into registers, NV pieces a thread. Resident blocks walk the rows with the
 // smoothing factors in registers, the next row's pieces on their way while a row is reduced and quantized (16,384
 // rows of 4,096 bfloat16, smoothed: 76 us with a block to a row and the factors loaded for each).
-// Blocks of 512 are held to registers for two an SM where that spills nothing (17,316 rows of 5,056 float: 101 us with
-// the product of 128 channels, 119 with one block).
+// The registers are held to four blocks of 128 an SM (16,384 rows of 4,096 bfloat16 and their product with 128 channels:
+// 46.6 us, 51.5 with the compiler's own choice) and, where that spills nothing, two of 512 (17,316 rows of 5,056
+// float: 101 us, 119 with one block).
 template <class T, int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR == 512 && (sizeof(T) == 4 || NV <= 2) ? 2 : 1)
+__global__ void __launch_bounds__(TPR < 128 ? 128 : TPR, TPR <= 128 ? 4 : (sizeof(T) == 4 || NV <= 2) ? 2 : 1)
     k_quant_rows(QuantArgs a) {
   constexpr int VE = kPiece<T>;
   constexpr int RPB = TPR < 128 ? 128 / TPR : 1;

@@ -19,6 +19,10 @@
 //          third less L2 traffic a product at 256 tokens, where that traffic is what one CTA alone waits for.
 //   SPLIT  a cluster of 2..8 CTAs splits the depth of one tile and adds the partial sums through distributed
 //          shared memory, where there are too few tiles for the SMs.
+// Device times and what bounds them: 16,384 x 8,192 x 4,096 to bfloat16 351 us (PAIR: 512 cycles a depth block, the
+// tensor pipe's rate, at the 1.3 GHz that the power cap leaves); 65,536 x 1,536 x 384 48 us (the epilogue, 3,200 cycles a
+// 256 x 256 tile against 1,536 of MMAs); 1 x 4,096 x 4,096 5 us, 1 x 18,944 x 4,096 16 us (the weights' bytes: 6.5 TB/s
+// beyond the first 4 us).
 #include <algorithm>
 #include <cmath>
 
@@ -210,10 +214,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0 && mine) mbar_arrive_expect_tx(red_full, uint32_t(g.split - 1) * mine * kChannels * 4);
   }
   __syncthreads();
-  if constexpr (MODE != ONE) {  // the peers' barriers and shared memory are there before anything reaches for them
-    cluster_arrive_release();
-    cluster_wait_acquire();
-  }
+  // the peers' barriers and shared memory are there before anything reaches for them: at once in a pair, when its partial
+  // sums leave in a split
+  if constexpr (MODE != ONE) cluster_arrive_release();
+  if constexpr (MODE == PAIR) cluster_wait_acquire();
   if (!g.early_w) pdl_wait();
   pdl_trigger();
   // the first blocks of weights are asked for before the kernel ahead (which quantizes the tokens) has ended
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   // TMEM only now: a CTA that still waits for the kernel ahead holds none, so that kernel can always get its own
   uint32_t tmem = 0;
-  if (warp >= 1) {
+  auto meet_tmem = [&] {  // warps 1..17: the allocation's address
     if (warp == 1) {
       if constexpr (MODE == PAIR) {
         tmem_alloc_pair(tmem_slot, S::TCOLS);
@@ -257,7 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     named_bar(1, kThreads - 32);
     tc_fence_after();
     tmem = *tmem_slot;
-  }
+  };
+  if (warp >= 1 && (!FUSE || warp == 1)) meet_tmem();
 
   if (warp == 0) {
     // ------------------------------------------------ TMA producer
@@ -342,7 +347,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int part4 = (warp - 2) >> 2;       // which quarter of the tokens
     constexpr int QW = BT / 4;               // tokens to a quarter
     const int ch = (warp & 3) * 32 + lane;   // channel within the CTA's 128 = TMEM lane
-    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     const int c0 = part4 * QW;
     float* as = s_scale + (warp - 2) * 32;   // scales of the 32 tokens at hand
     // Each warp keeps its own scales and biases: a lane's channel's, and those of tokens lane and lane + 32 of
@@ -398,8 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       fence_proxy_async();
       mbar_arrive(tok_full);
-      named_bar(6, 32 * kEpi);
+      meet_tmem();  // the tokens' scales are there for every warp too
     }
+    const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
     bool ok = true;
     int it = 0;
     for (; more; ++it) {
@@ -566,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < QW; ++j) part[(c0 + j) * kChannels + ch] = int(r[j]);
         }
         fence_proxy_async();
+        cluster_wait_acquire();
         named_bar(6, 32 * kEpi);
         if (ok && et < g.split && et != int(rank)) {
           const int count = max(0, min(run, mv - et * run));
@@ -591,6 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   __syncwarp();
+  if (MODE == SPLIT && warp < 2) cluster_wait_acquire();
   tc_fence_before();
   __syncthreads();
   if constexpr (MODE != ONE) {  // no CTA leaves while another may still reach into it

@@ -54,7 +54,7 @@ enum Mode { ONE = 0, PAIR = 1, SPLIT = 2 };
 
 // FUSE: the most depth blocks of quantized tokens a CTA holds (16 tokens, 2 KB a block).
 constexpr int kFuseBlocks = 32;
-constexpr size_t kFuseMost = 8 << 10;          // bytes of activations
+constexpr size_t kFuseMost = 16 << 10;         // bytes of activations
 
 template <int BT, int MODE, bool FUSE = false>
 struct Shape {
@@ -797,8 +797,8 @@ size_t product_scratch(const ProductArgs& a) {
 }
 
 // Up to 16 tokens whose depth (its share of a split) fits a CTA's token blocks, and little enough to read in each of
-// some 130 CTAs at once. On the device one 4,096-deep bfloat16 token takes 6.7 us this way and 6.7 us in two kernels,
-// two smoothed ones 7.6 and 6.8, sixteen 11.8 and 7.0; a launch less spares the host about 2 us.
+// some 130 CTAs at once. On the device one 4,096-deep bfloat16 token takes 6.3 us this way and 6.7 us in two kernels,
+// two smoothed ones 7.3 and 6.8, sixteen 11.6 and 7.1; a launch less spares the host about 2 us.
 int launch_product_fused(const ProductArgs& args, const QuantArgs& q, cudaStream_t st) {
   ProductArgs a = args;
   if (a.M > 16 || size_t(a.M) * a.K * float_type_bytes(q.x_type) > kFuseMost || !in_place(a.w, a.ldw, a.N)) return 1;

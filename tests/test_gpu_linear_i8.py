@@ -187,7 +187,7 @@ def run_linear(eng, M, N, K, x_type, dtype, seed, smooth=True, bias=True, x_pitc
 
 
 @pytest.mark.parametrize("x_type", TYPES)
-@pytest.mark.parametrize("M,N,K", [(1, 384, 384), (1, 129, 4096), (2, 64, 1), (7, 100, 1003), (16, 1536, 384),
+@pytest.mark.parametrize("M,N,K", [(1, 384, 384), (1, 1, 64), (2, 3, 130), (5, 1, 1003), (1, 129, 4096), (2, 64, 1), (7, 100, 1003), (16, 1536, 384),
                                    (17, 40, 1536), (64, 384, 1536), (130, 257, 2050), (509, 1001, 1003), (1, 16, 20001),
                                    (3, 128, 16392), (600, 384, 4104)])
 def test_linear(eng, x_type, M, N, K):
@@ -371,4 +371,42 @@ def test_refusals(eng):
         eng.matmul_i8(torch.empty(1, 0, dtype=torch.int8, device="cuda"), a_s[:1],
                       torch.empty(N, 0, dtype=torch.int8, device="cuda"), w_s, out[:1])
     assert e.value.code == -1
+    eng.sync()
+
+
+def test_refusals_of_the_c_abi(eng):
+    """Status -1 and a message, whatever the argument; nothing is launched."""
+    from arctic_embed_s_int8 import _lib
+
+    lib, h = _lib.lib(), eng.handle
+    M, N, K = 4, 32, 48
+    a, w, a_s, w_s, b = (dev(x) for x in make(M, N, K, 1))
+    x, out = torch.zeros(M, K, device="cuda"), torch.full((M, N), 3.0, device="cuda")
+    p = {"a": a.data_ptr(), "as": a_s.data_ptr(), "w": w.data_ptr(), "ws": w_s.data_ptr(), "b": b.data_ptr(),
+         "o": out.data_ptr(), "x": x.data_ptr()}
+
+    def matmul(M=M, N=N, K=K, a=p["a"], lda=K, a_s=p["as"], w=p["w"], ldw=K, w_s=p["ws"], b=p["b"], t=0, o=p["o"], ldo=N):
+        return lib.ae_matmul_i8(h, M, N, K, a, lda, a_s, w, ldw, w_s, b, t, o, ldo)
+
+    def linear(xt=0, x=p["x"], ldx=K, s=None, **kw):
+        v = dict(M=M, N=N, K=K, w=p["w"], ldw=K, w_s=p["ws"], b=p["b"], t=0, o=p["o"], ldo=N) | kw
+        return lib.ae_linear_i8(h, v["M"], v["N"], v["K"], xt, x, ldx, s, v["w"], v["ldw"], v["w_s"], v["b"], v["t"],
+                                v["o"], v["ldo"])
+
+    shared = [dict(N=0), dict(K=0), dict(K=131072, ldw=131072), dict(M=2 ** 30 + 1), dict(N=2 ** 30 + 1), dict(w=None),
+              dict(w_s=None), dict(o=None), dict(t=3), dict(t=-1), dict(ldw=K - 1), dict(ldo=N - 1),
+              dict(ldo=2 ** 39), dict(ldw=2 ** 39), dict(w_s=p["ws"] + 2), dict(b=p["b"] + 1), dict(o=p["o"] + 2)]
+    launches = eng.kernel_launches()
+    for kw in shared + [dict(a=None), dict(a_s=None), dict(lda=K - 1), dict(lda=2 ** 39), dict(a_s=p["as"] + 1)]:
+        assert matmul(**({"lda": kw["K"]} if "K" in kw else {}) | kw) == -1, kw
+        assert b"ae_matmul_i8" in lib.ae_last_error(h)
+    for kw in shared + [dict(x=None), dict(xt=4), dict(ldx=K - 1), dict(ldx=2 ** 39), dict(x=p["x"] + 2),
+                        dict(s=p["b"] + 2)]:
+        assert linear(**({"ldx": kw["K"]} if "K" in kw else {}) | kw) == -1, kw
+        assert b"ae_linear_i8" in lib.ae_last_error(h)
+    assert matmul(M=0, a=None, a_s=None, o=None) == 0 and linear(M=0, x=None, o=None) == 0
+    assert eng.kernel_launches() == launches
+    eng.sync()
+    assert (out == 3).all()
+    assert matmul() == 0 and linear() == 0
     eng.sync()

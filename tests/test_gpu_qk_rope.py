@@ -235,3 +235,41 @@ def test_refusals(eng):
         eng.qk_norm_rope(wide, wide, torch.empty_like(wide), torch.empty_like(wide))
     assert e.value.code == -1
     eng.sync()
+
+
+def test_no_tokens(eng):
+    for T, Hq, Hk in ((0, 2, 1), (3, 0, 0)):
+        q, k = torch.empty(T, Hq, 32, device="cuda"), torch.empty(T, Hk, 32, device="cuda")
+        eng.qk_norm_rope(q, k, q, k, dev(rope_table(8, 32)), positions=torch.zeros(T, dtype=torch.int32, device="cuda"))
+    eng.sync()
+
+
+def test_refusals_of_the_c_abi(eng):
+    """Status -1 and a message, whatever the argument; nothing is launched."""
+    from arctic_embed_s_int8 import _lib
+
+    lib, h, T, D = _lib.lib(), eng.handle, 4, 32
+    x, table = torch.full((T, 2, D), 3.0, device="cuda"), dev(rope_table(8, D))
+    pos = torch.zeros(T, dtype=torch.int32, device="cuda")
+    P, S = x.data_ptr(), (2 * D, D)
+
+    def call(type=0, T=T, Hq=1, Hk=1, D=D, R=D, flags=0, q=(P, *S), k=(P + 4 * D, *S), qo=(P, *S), ko=(P + 4 * D, *S),
+             qw=None, kw=None, eps=1e-6, table=table.data_ptr(), rows=8, pos=pos.data_ptr(), cu=None, n=0):
+        return lib.ae_qk_norm_rope(h, type, T, Hq, Hk, D, R, flags, *q, *k, *qo, *ko, qw, kw, eps, table, rows, pos, cu, n)
+
+    launches = eng.kernel_launches()
+    null = (None, *S)
+    for kw in (dict(type=3), dict(type=-1), dict(flags=4), dict(D=0, R=0), dict(D=513, R=0), dict(R=34), dict(R=31),
+               dict(Hq=65536), dict(T=2 ** 30 + 1), dict(eps=-1.0), dict(eps=float("nan")), dict(q=null), dict(k=null),
+               dict(qo=null), dict(ko=null), dict(table=None), dict(rows=0), dict(pos=None), dict(rows=2 ** 31),
+               dict(pos=None, cu=pos.data_ptr(), n=0), dict(q=(P + 2, *S)), dict(qw=P + 1), dict(pos=pos.data_ptr() + 2),
+               dict(k=(P, 2 ** 32, D))):
+        assert call(**kw) == -1, kw
+        assert b"ae_qk_norm_rope" in lib.ae_last_error(h)
+    assert call(T=0, q=null, k=null, qo=null, ko=null, pos=None) == 0
+    assert call(Hq=0, Hk=0) == 0
+    assert eng.kernel_launches() == launches
+    eng.sync()
+    assert (x == 3).all()
+    assert call() == 0
+    eng.sync()

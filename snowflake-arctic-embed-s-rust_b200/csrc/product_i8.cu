@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       // the four warps of a quarter write their channels of a token together: whole stretches of the output's rows
-      // reach L2 and memory close in time (13,944 x 10,515 float, K = 128: 231 us apart, 167 together)
+      // reach L2 and memory close in time (13,944 x 10,515 float, K = 128: 192 us apart, 131 together)
       named_bar(2 + part4, 128);
       // before the columns from c on: the scales of their 32 tokens
       auto scales = [&](int c) {
@@ -714,8 +714,8 @@ int room_for(int split) {
   return n;
 }
 
-// The tile by an estimate of the device time in cycles, whose parts are fits of measurements over 22 shapes (it
-// picks the fastest or within 5 % of it in all of them):
+// The tile by an estimate of the device time in cycles, whose parts are fits of measurements (over 36 shapes and
+// types it takes the fastest tile or one within 5 % of it in 27, within 12 % in all):
 //   block   128 bytes of depth of one tile: its MMAs (8,192 products a cycle); 145 cycles and its bytes at 125 a
 //           cycle for a CTA alone; its share of the 62 bytes a cycle and SM that L2 gives when all SMs read
 //   tile    `blocks` of them, or its epilogue where that takes longer: 400 cycles and 15 a token of 16-bit results, 22

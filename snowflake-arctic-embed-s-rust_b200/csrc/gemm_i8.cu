@@ -808,7 +808,7 @@ int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_ro
 int make_tmap_store(CUtensorMap* map, void* base, size_t rows, size_t cols, size_t pitch, int elem_bytes, int box_rows) {
   auto enc = get_encode();
   if (!enc) return -1;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || (pitch % 16) || rows == 0) return -2;
+  if ((reinterpret_cast<uintptr_t>(base) & 15) || pitch % 16 || cols * elem_bytes % 16 || rows == 0) return -2;
   cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)};
   cuuint64_t strides[1] = {cuuint64_t(pitch)};
   cuuint32_t box[2] = {32, cuuint32_t(box_rows)};

@@ -41,7 +41,8 @@ int make_tmap_i8(CUtensorMap* map, const void* base, int rows, int K, int box_ro
 // The same for rows `pitch` bytes apart (a multiple of 16); K may be any, bytes past it read as zero.
 int make_tmap_i8_rows(CUtensorMap* map, const void* base, size_t rows, size_t K, size_t pitch, int box_rows);
 // Tensor map for storing a [rows, cols] row-major matrix of 16-bit (64-byte swizzle) or 32-bit (128-byte
-// swizzle) elements, rows `pitch` bytes apart (base and pitch multiples of 16), in boxes of 32 columns.
+// swizzle) elements, rows `pitch` bytes apart (base, pitch and a row's bytes multiples of 16: a row's last 16 bytes
+// are stored whole), in boxes of 32 columns.
 int make_tmap_store(CUtensorMap* map, void* base, size_t rows, size_t cols, size_t pitch, int elem_bytes, int box_rows);
 int num_sms();  // of the current device
 constexpr int kBoxA = 128;

@@ -629,10 +629,11 @@ __global__ void __launch_bounds__(256) k_lay_rows(const int8_t* src, size_t ld, 
   }
 }
 
-// Whether TMA can store to the output.
+// Whether TMA can store to the output: rows that start and end on 16 bytes (a store's last 16 bytes of a row are
+// written whole, past the map's end too).
 bool can_box(const ProductArgs& a) {
-  const size_t pitch = a.ldo * float_type_bytes(a.out_type);
-  return (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && pitch % 16 == 0 && pitch >> 40 == 0;
+  const size_t size = float_type_bytes(a.out_type), pitch = a.ldo * size;
+  return (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && pitch % 16 == 0 && a.N * size % 16 == 0 && pitch >> 40 == 0;
 }
 
 // Token tiles walked together. One after the other the CTAs at work write neighbouring stretches of the same

@@ -114,6 +114,14 @@ def test_pitches_and_offsets(eng, M, a_pitch, a_lead, w_pitch, w_lead):
                    w=lambda x: pitched(torch.from_numpy(x), w_pitch, w_lead))
 
 
+@pytest.mark.parametrize("M,N,K,pitch", [(1500, 1031, 640, 1032), (4099, 1025, 200, 1040), (300, 8190, 384, 8200),
+                                         (6000, 397, 130, 400)])
+def test_rows_that_end_inside_16_bytes(eng, M, N, K, pitch):
+    """Outputs whose rows start on 16 bytes and end elsewhere: what follows a row's end is not written."""
+    for i, dt in enumerate(TYPES):
+        run_matmul(eng, M, N, K, dt, M + N + i, pitch=pitch)
+
+
 @pytest.mark.parametrize("M", [1, 130])
 def test_largest_sums(eng, M):
     """-128 * -128 over the deepest product is just inside int32."""

@@ -122,6 +122,49 @@ def test_rows_that_end_inside_16_bytes(eng, M, N, K, pitch):
         run_matmul(eng, M, N, K, dt, M + N + i, pitch=pitch)
 
 
+def far(x, pitch):
+    """x in rows `pitch` elements apart, in a buffer that is not cleared."""
+    r, c = x.shape
+    view = torch.empty((r - 1) * pitch + c, dtype=x.dtype, device="cuda").as_strided((r, c), (pitch, 1))
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("pitch", [2 ** 30, 2 ** 30 + 1])
+def test_offsets_beyond_32_bits(eng, pitch):
+    """Rows 2^30 elements apart, read in place or laid out first, and results stored as far apart."""
+    M, N, K = 5, 200, 130
+    a, w, a_s, w_s, b = make(M, N, K, 7)
+    out = torch.empty(2 * pitch + N, dtype=torch.float16, device="cuda").as_strided((3, N), (pitch, 1))
+    eng.matmul_i8(dev(a[:3]), dev(a_s[:3]), dev(w), dev(w_s), out, bias=dev(b))
+    eng.sync()
+    check(out, a[:3], a_s[:3], w, w_s, b)
+    del out
+    near = torch.empty(M, 5, dtype=torch.float32, device="cuda")
+    eng.matmul_i8(far(torch.from_numpy(a), pitch), dev(a_s), far(torch.from_numpy(w[:5]), pitch), dev(w_s[:5]), near)
+    eng.sync()
+    check(near, a, a_s, w[:5], w_s[:5], None)
+    x = torch.randn(3, K, dtype=torch.float16, device="cuda")
+    here, there = (torch.empty(3, N, dtype=torch.float32, device="cuda") for _ in range(2))
+    eng.linear_i8(x, dev(w), dev(w_s), here)
+    eng.linear_i8(far(x, pitch), dev(w), dev(w_s), there)
+    eng.sync()
+    assert torch.equal(here, there)
+
+
+@pytest.mark.parametrize("N", [58000, 58001])
+def test_outputs_beyond_32_bits(eng, N):
+    """2.3 billion results, as boxes and from the lanes: rows from all over them."""
+    M, K = 40000, 40
+    a, w, a_s, w_s, b = make(M, N, K, 8)
+    out = torch.full((M, N), float("nan"), dtype=torch.bfloat16, device="cuda")
+    eng.matmul_i8(dev(a), dev(a_s), dev(w), dev(w_s), out, bias=dev(b))
+    eng.sync()
+    assert not out[::97].isnan().any()
+    rows = [0, 255, 256, 18511, 18512, 37025, 37026, 37027, 39998, 39999]
+    check(out[rows], a[rows], a_s[rows], w, w_s, b)
+
+
 @pytest.mark.parametrize("M", [1, 130])
 def test_largest_sums(eng, M):
     """-128 * -128 over the deepest product is just inside int32."""

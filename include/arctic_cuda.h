@@ -182,8 +182,7 @@ enum { AE_F32 = 0, AE_F16 = 1, AE_BF16 = 2 };
  * [M, N] of out_type. The sum is exact (int32, hence K <= 131,071); the result is rounded to out_type once.
  * lda, ldw (bytes) and ldo (elements) are the rows' pitches, at least the rows' lengths. Any M (0: nothing
  * is done), N and K. Operands that start on 16 bytes with a pitch that is a multiple of 16 are read where
- * they are; others are first laid out so in scratch that the context keeps for each stream (grown on
- * demand, which synchronises the stream; run once before a stream capture). out overlaps no operand. */
+ * they are; others are first laid out so in scratch (ae_release_scratch). out overlaps no operand. */
 int ae_matmul_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_a, uint64_t lda,
                  const float* d_a_scale, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
                  const float* d_bias, int out_type, void* d_out, uint64_t ldo);
@@ -197,6 +196,16 @@ int ae_matmul_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, const int8_t* 
 int ae_linear_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, int x_type, const void* d_x, uint64_t ldx,
                  const float* d_inv_smooth, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
                  const float* d_bias, int out_type, void* d_out, uint64_t ldo);
+
+/* Scratch of ae_matmul_i8 and ae_linear_i8. The context keeps one block for each stream that it was set to, grown on
+ * demand, which synchronises the stream. A call that is captured takes a block of the graph's own instead, so neither
+ * later calls, larger or not, nor other graphs touch what its replays use, on whatever streams they run. The block
+ * serves other captures once the graph and everything instantiated from it are destroyed; graphs must not be replayed
+ * after ae_ctx_destroy. Run a call once before capturing it all the same: its first use loads its kernels.
+ * This call waits for the present stream and frees its block and those of graphs that are gone. Call it
+ * before destroying a stream that the context was set to, whose block stays until ae_ctx_destroy otherwise; not while
+ * the stream is being captured. */
+int ae_release_scratch(ae_ctx* ctx);
 
 /* RMS norm of every query and key head, and the rotation of its first rotary_dim dims by the token's
  * position, in one pass:

@@ -120,6 +120,7 @@ extern "C" {
     pub fn ae_linear_i8(ctx: *mut ae_ctx, m: u32, n: u32, k: u32, x_type: c_int, d_x: *const c_void, ldx: u64,
                         d_inv_smooth: *const f32, d_w: *const i8, ldw: u64, d_w_scale: *const f32,
                         d_bias: *const f32, out_type: c_int, d_out: *mut c_void, ldo: u64) -> c_int;
+    pub fn ae_release_scratch(ctx: *mut ae_ctx) -> c_int;
     pub fn ae_qk_norm_rope(ctx: *mut ae_ctx, dtype: c_int, tokens: u32, q_heads: u32, k_heads: u32, head_dim: u32,
                            rotary_dim: u32, flags: c_int, d_q: *const c_void, q_token_stride: u64,
                            q_head_stride: u64, d_k: *const c_void, k_token_stride: u64, k_head_stride: u64,

@@ -208,6 +208,11 @@ class Engine:
         if code:
             self._check(code)
 
+    def release_scratch(self) -> None:
+        """ae_release_scratch: waits for the engine's present stream and frees the scratch that matmul_i8 and
+        linear_i8 keep for it, and that of captured graphs which are gone. For streams about to be destroyed."""
+        self._check(lib().ae_release_scratch(self._h))
+
     QK_NEIGHBOURS, QK_NO_NORM = 1, 2
 
     def qk_norm_rope(self, q, k, q_out, k_out, table=None, positions=None, cu=None, q_weight=None, k_weight=None,

@@ -37,6 +37,7 @@ SYMBOLS = [
     "ae_tokenizer_vocab_size", "ae_tokenizer_last_error", "ae_tokenize", "ae_tokenize_batch",
     "ae_selftest_wait_timeout", "ae_set_attention_mode", "ae_get_attention_mode", "ae_attention_i8",
     "ae_trace_forward", "ae_measure_int8_peak", "ae_matmul_i8", "ae_linear_i8", "ae_qk_norm_rope",
+    "ae_release_scratch",
 ]
 
 
@@ -117,6 +118,7 @@ def lib():
     u64 = C.c_uint64
     L.ae_matmul_i8.argtypes = [P, u32, u32, u32, P, u64, P, P, u64, P, P, C.c_int, P, u64]
     L.ae_linear_i8.argtypes = [P, u32, u32, u32, C.c_int, P, u64, P, P, u64, P, P, C.c_int, P, u64]
+    L.ae_release_scratch.argtypes = [P]
     L.ae_qk_norm_rope.argtypes = ([P, C.c_int, u32, u32, u32, u32, u32, C.c_int] + [P, u64, u64] * 4 +
                                   [P, P, C.c_float, P, u32, P, P, u32])
     L.ae_tokenizer_create_from_file.argtypes = [C.c_char_p, C.POINTER(P)]

@@ -40,6 +40,7 @@
 #include "linear_i8.h"
 #include "ptx.cuh"
 #include "rowmath.cuh"
+#include "scratch.h"
 
 using namespace ae;
 
@@ -123,13 +124,7 @@ struct ae_ctx {
   uint32_t* d_cu_single = nullptr;  // [513][2]: {0, L} at 2L, the cu_seqlens of one sequence of L ids
   float* d_gemm_scratch = nullptr;  // ae_gemm_i8's split LayerNorm path: h of up to gemm_scratch_rows rows
   uint32_t gemm_scratch_rows = 0;
-  // scratch of ae_matmul_i8 / ae_linear_i8, one for each stream the context was set to, so that a call
-  // on one stream never writes what a call on another may still be reading
-  struct Scratch {
-    uint8_t* p = nullptr;
-    size_t bytes = 0;
-  };
-  std::map<cudaStream_t, Scratch> scratch;
+  ae::StreamScratch scratch;  // of ae_matmul_i8 / ae_linear_i8
   bool has_model = false;
   DevModel model;
   void* h_model = nullptr;  // pinned host image of the model arena (reused across loads)
@@ -1160,8 +1155,7 @@ int ae_ctx_destroy(ae_ctx* c) {
   if (c->h_err) cudaFreeHost(c->h_err);
   if (c->d_cu_single) cudaFree(c->d_cu_single);
   if (c->d_gemm_scratch) cudaFree(c->d_gemm_scratch);
-  for (auto& s : c->scratch)
-    if (s.second.p) cudaFree(s.second.p);
+  c->scratch.close();
   if (c->own_stream) cudaStreamDestroy(c->own_stream);
   delete c;
   return 0;
@@ -1689,22 +1683,10 @@ int ae_attention_i8(ae_ctx* c, const float* d_qkv, const uint32_t* d_cu, uint32_
 
 namespace {
 
-// Scratch of at least `bytes` for the context's present stream (grown by half again, never shrunk).
+// Scratch of at least `bytes` for a call on the context's present stream.
 int stream_scratch(ae_ctx* c, size_t bytes, uint8_t** out) {
   try {
-    auto& s = c->scratch[c->stream];
-    if (s.bytes < bytes) {
-      if (s.p) {
-        CUDA_TRY(c, cudaStreamSynchronize(c->stream));
-        cudaFree(s.p);
-        s.p = nullptr;
-      }
-      const size_t want = std::max(bytes, s.bytes + s.bytes / 2);
-      s.bytes = 0;
-      CUDA_TRY(c, cudaMalloc(&s.p, want));
-      s.bytes = want;
-    }
-    *out = s.p;
+    CUDA_TRY(c, c->scratch.take(c->stream, bytes, out));
     return 0;
   } catch (const std::bad_alloc&) {
     return fail(c, AE_ERR_CUDA, "out of host memory");
@@ -1813,6 +1795,17 @@ int ae_linear_i8(ae_ctx* c, uint32_t M, uint32_t N, uint32_t K, int x_type, cons
   a.a = q.q;
   a.a_scale = q.scale;
   return product(c, a, scratch + q_bytes + s_bytes, 1);
+}
+
+int ae_release_scratch(ae_ctx* c) {
+  if (!c) return AE_ERR_INVALID_ARG;
+  DeviceGuard g(c->device);
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  CUDA_TRY(c, cudaStreamIsCapturing(c->stream, &status));
+  if (status != cudaStreamCaptureStatusNone)
+    return fail(c, AE_ERR_INVALID_ARG, "ae_release_scratch: the stream is being captured");
+  CUDA_TRY(c, c->scratch.release(c->stream));
+  return 0;
 }
 
 int ae_qk_norm_rope(ae_ctx* c, int type, uint32_t tokens, uint32_t q_heads, uint32_t k_heads, uint32_t head_dim,

@@ -113,7 +113,8 @@ int64_t whole(PyObject* o) {
   return v;
 }
 
-// The C call without the interpreter's lock, as ctypes makes it.
+// The C call without the interpreter's lock, as ctypes makes it. `call` holds plain values: a tensor that is asked for its
+// address throws where it has none, which needs the lock.
 template <class F>
 PyObject* unlocked(F&& call) {
   int code;
@@ -156,9 +157,11 @@ PyObject* matmul_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const float* a_scale = at_address<const float>(vector(args[3], "a_scale", M, at::kFloat, dev));
     const float* w_scale = at_address<const float>(vector(args[5], "w_scale", N, at::kFloat, dev));
     const float* bias = floats_or_none(args[7], "bias", N, dev);
-    return unlocked([&] {
-      return g_matmul(ctx, count(M), count(N), count(K), at_address<const int8_t>(a), pitch(a), a_scale,
-                      at_address<const int8_t>(w), pitch(w), w_scale, bias, out_type, out.data_ptr(), pitch(out));
+    const int8_t *pa = at_address<const int8_t>(a), *pw = at_address<const int8_t>(w);
+    void* po = out.data_ptr();
+    const uint64_t lda = pitch(a), ldw = pitch(w), ldo = pitch(out);
+    return unlocked([=] {
+      return g_matmul(ctx, count(M), count(N), count(K), pa, lda, a_scale, pw, ldw, w_scale, bias, out_type, po, ldo);
     });
   });
 }
@@ -179,9 +182,12 @@ PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const float* smooth = floats_or_none(args[3], "inv_smooth", K, dev);
     const float* w_scale = at_address<const float>(vector(args[5], "w_scale", N, at::kFloat, dev));
     const float* bias = floats_or_none(args[7], "bias", N, dev);
-    return unlocked([&] {
-      return g_linear(ctx, count(M), count(N), count(K), x_type, x.data_ptr(), pitch(x), smooth,
-                      at_address<const int8_t>(w), pitch(w), w_scale, bias, out_type, out.data_ptr(), pitch(out));
+    const int8_t* pw = at_address<const int8_t>(w);
+    void *px = x.data_ptr(), *po = out.data_ptr();
+    const uint64_t ldx = pitch(x), ldw = pitch(w), ldo = pitch(out);
+    return unlocked([=] {
+      return g_linear(ctx, count(M), count(N), count(K), x_type, px, ldx, smooth, pw, ldw, w_scale, bias, out_type, po,
+                      ldo);
     });
   });
 }
@@ -246,7 +252,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(args[11]);
     if (eps == -1.0 && PyErr_Occurred()) throw Refused{};
     const int flags = int(whole(args[12]));
-    return unlocked([&] {
+    return unlocked([=] {
       return g_qk(ctx, type, count(T), count(Hq), count(Hk), count(D), count(rotary), flags, q.p, q.token, q.head, k.p,
                   k.token, k.head, qo.p, qo.token, qo.head, ko.p, ko.token, ko.head, qw, kw, float(eps), table,
                   count(rows), positions, cu, count(seqs));

@@ -1,0 +1,54 @@
+"""The general operators' calls on torch tensors that hold no memory of a GPU, or not what their address says."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from conftest import PKG, ROOT
+
+# Tensors of cuda:0 without a GPU: `plain` ones have the address 0, which the C ABI would refuse (as it does the null context),
+# and those in a batch, as torch.func.vmap passes them, have none and throw when asked for it.
+HOLLOW = """
+import torch
+from torch._C._functorch import _add_batch_dim
+from arctic_embed_s_int8 import _lib
+
+class Hollow(torch.Tensor):
+    @staticmethod
+    def __new__(cls, *size, dtype=torch.float32):
+        return torch.Tensor._make_wrapper_subclass(cls, size, dtype=dtype, device="cuda:0")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError(str(func))
+
+def batched(*size, dtype=torch.float32):
+    return _add_batch_dim(Hollow(3, *size, dtype=dtype), 0, 1)
+
+m = _lib.tensors()
+"""
+
+
+def run(lines: str) -> str:
+    """What a process of its own prints."""
+    r = subprocess.run([sys.executable, "-c", HOLLOW + lines], capture_output=True, text=True, cwd=ROOT,
+                       env={**os.environ, "PYTHONPATH": PKG})
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr[-500:])
+    return r.stdout
+
+
+@pytest.mark.parametrize("call,args", [
+    ("matmul_i8", ["Hollow(2, 8, dtype=i8)", "Hollow(2)", "Hollow(4, 8, dtype=i8)", "Hollow(4)", "Hollow(2, 4)", "None"]),
+    ("linear_i8", ["Hollow(2, 8)", "Hollow(8)", "Hollow(4, 8, dtype=i8)", "Hollow(4)", "Hollow(2, 4)", "Hollow(4)"]),
+    ("qk_norm_rope", ["Hollow(2, 3, 8)", "Hollow(2, 1, 8)", "Hollow(2, 3, 8)", "Hollow(2, 1, 8)", "Hollow(5, 4)",
+                      "Hollow(2, dtype=torch.int32)", "None", "Hollow(8)", "Hollow(8)", "1e-6", "0"])])
+def test_tensors_without_an_address_raise(call, args):
+    """Whichever operand it is, and with the interpreter's lock held (the process ends otherwise)."""
+    lines = f"i8 = torch.int8\nassert m.{call}(0, 0, {', '.join(args)}) == -1\n"
+    for i, a in enumerate(args):
+        if "Hollow" not in a:
+            continue
+        one = [*args[:i], a.replace("Hollow", "batched"), *args[i + 1:]]
+        lines += f"try:\n    m.{call}(0, 0, {', '.join(one)})\nexcept RuntimeError as e:\n    print('storage' in str(e))\n"
+    assert run(lines).split() == ["True"] * sum("Hollow" in a for a in args)

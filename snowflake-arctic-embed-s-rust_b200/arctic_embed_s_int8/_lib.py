@@ -71,8 +71,15 @@ class ModelDesc(C.Structure):
 
 
 def build(force: bool = False) -> str:
-    """Compiles the CUDA library for sm_100a and the module of its calls on torch tensors (make in csrc/)."""
-    subprocess.run(["make", "-s", "-C", CSRC, "-j4", "python", f"PYTHON={sys.executable}"], check=True)
+    """Compiles the CUDA library for sm_100a (make in csrc/) and, where there is a torch, the module of its calls on
+    torch tensors."""
+    try:
+        import torch  # noqa: F401
+
+        targets = ["python", f"PYTHON={sys.executable}"]
+    except ImportError:
+        targets = []
+    subprocess.run(["make", "-s", "-C", CSRC, "-j8", *targets], check=True)
     return LIB_PATH
 
 

@@ -12,7 +12,6 @@ import sys
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libarctic_cuda.so")
-TENSORS_PATH = os.path.join(_PKG_ROOT, "lib", "arctic_tensors.so")
 CSRC = os.path.join(_PKG_ROOT, "csrc")
 HEADER = os.path.join(os.path.dirname(_PKG_ROOT), "include", "arctic_cuda.h")
 
@@ -154,17 +153,26 @@ def check(ctx, code: int) -> None:
 _tensors = None
 
 
+def tensors_path() -> str:
+    """Where the module of the calls on torch tensors lies: it reads the tensors of one torch in one interpreter, and is
+    named after both."""
+    import sysconfig
+
+    import torch
+
+    return os.path.join(_PKG_ROOT, "lib", f"arctic_tensors-torch{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
 def tensors():
     """The module of the general operators' calls on torch tensors (csrc/tensors.cpp), bound to lib()."""
     global _tensors
     if _tensors is None:
         import importlib.util
 
-        import torch  # noqa: F401  (its libraries, which the module uses)
-
-        if not os.path.exists(TENSORS_PATH):
-            raise RuntimeError(f"{TENSORS_PATH} is missing: build it with `make -C {CSRC} python`")
-        spec = importlib.util.spec_from_file_location("arctic_tensors", TENSORS_PATH)
+        path = tensors_path()  # which imports torch, whose libraries the module uses
+        if not os.path.exists(path):
+            raise RuntimeError(f"{path} is missing: build it with `make -C {CSRC} python PYTHON={sys.executable}`")
+        spec = importlib.util.spec_from_file_location("arctic_tensors", path)
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.bind(*(C.cast(getattr(lib(), n), C.c_void_p).value for n in ("ae_matmul_i8", "ae_linear_i8", "ae_qk_norm_rope")))

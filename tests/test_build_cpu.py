@@ -33,3 +33,20 @@ def test_build_without_torch(tree):
                      "try:\n    _lib.tensors()\nexcept ImportError as e:\n    print(e)\n", [tree / "without"])
     assert r.returncode == 0, r.stderr[-800:]
     assert "no torch here" in r.stdout
+
+
+def test_module_of_another_torch_is_not_used(tree):
+    """A module is built for one torch and one interpreter: after a change of either, make builds another, and one that
+    is not there is asked for rather than another loaded."""
+    build = "from arctic_embed_s_int8 import _lib; _lib.build(); print(_lib.tensors().__file__)"
+    first = python(tree, build)
+    assert first.returncode == 0, first.stderr[-800:]
+    # the same torch under another version's name
+    (tree / "other").mkdir()
+    (tree / "other" / "sitecustomize.py").write_text("import torch\ntorch.__version__ += '.other'\n")
+    missing = python(tree, "from arctic_embed_s_int8 import _lib; _lib.tensors()", [tree / "other"])
+    assert missing.returncode != 0 and "is missing" in missing.stderr
+    second = python(tree, build, [tree / "other"])
+    assert second.returncode == 0, second.stderr[-800:]
+    assert second.stdout != first.stdout
+    assert python(tree, build).stdout == first.stdout

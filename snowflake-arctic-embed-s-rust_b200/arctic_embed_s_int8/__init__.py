@@ -196,7 +196,8 @@ class Engine:
     def matmul_i8(self, a, a_scale, w, w_scale, out, bias=None) -> None:
         """ae_matmul_i8: out[m, n] = (sum_k a[m, k] w[n, k]) * (a_scale[m] * w_scale[n]) + bias[n] on device
         tensors: a [M, K] and w [N, K] int8, a_scale [M], w_scale [N] and bias [N] float32, out [M, N]
-        float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream."""
+        float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream. Computes no
+        gradients (nor do linear_i8 and qk_norm_rope): tensors that require them are refused unless grad mode is off."""
         code = tensors().matmul_i8(self._h.value, self.device, a, a_scale, w, w_scale, out, bias)
         if code:
             self._check(code)

@@ -6,6 +6,7 @@
 // does not fit, and returns the C ABI's status code. bind() receives the C functions' addresses, so that this
 // module and the ctypes binding use one loaded library.
 #include <Python.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -28,7 +29,16 @@ struct Refused {};  // a Python exception is set
 
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) refuse("%s must be a torch tensor%s", what);
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  // as torch refuses operations with out=: a gradient would end here without a word
+  if (t.requires_grad() && c10::GradMode::is_enabled())
+    refuse("%s requires grad, but no gradients are computed: call this under torch.no_grad()%s", what);
+  return t;
+}
+
+// For autograd, which otherwise takes what it saved of a result for what it still holds.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 const char* type_name(at::ScalarType t) {
@@ -116,12 +126,12 @@ int64_t whole(PyObject* o) {
 // The C call without the interpreter's lock, as ctypes makes it. `call` holds plain values: a tensor that is asked for its
 // address throws where it has none, which needs the lock.
 template <class F>
-PyObject* unlocked(F&& call) {
+int unlocked(F&& call) {
   int code;
   Py_BEGIN_ALLOW_THREADS;
   code = call();
   Py_END_ALLOW_THREADS;
-  return PyLong_FromLong(code);
+  return code;
 }
 
 template <class F>
@@ -160,9 +170,11 @@ PyObject* matmul_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int8_t *pa = at_address<const int8_t>(a), *pw = at_address<const int8_t>(w);
     void* po = out.data_ptr();
     const uint64_t lda = pitch(a), ldw = pitch(w), ldo = pitch(out);
-    return unlocked([=] {
+    const int code = unlocked([=] {
       return g_matmul(ctx, count(M), count(N), count(K), pa, lda, a_scale, pw, ldw, w_scale, bias, out_type, po, ldo);
     });
+    if (code == AE_OK) written(out);
+    return PyLong_FromLong(code);
   });
 }
 
@@ -185,10 +197,12 @@ PyObject* linear_i8(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int8_t* pw = at_address<const int8_t>(w);
     void *px = x.data_ptr(), *po = out.data_ptr();
     const uint64_t ldx = pitch(x), ldw = pitch(w), ldo = pitch(out);
-    return unlocked([=] {
+    const int code = unlocked([=] {
       return g_linear(ctx, count(M), count(N), count(K), x_type, px, ldx, smooth, pw, ldw, w_scale, bias, out_type, po,
                       ldo);
     });
+    if (code == AE_OK) written(out);
+    return PyLong_FromLong(code);
   });
 }
 
@@ -252,11 +266,16 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(args[11]);
     if (eps == -1.0 && PyErr_Occurred()) throw Refused{};
     const int flags = int(whole(args[12]));
-    return unlocked([=] {
+    const int code = unlocked([=] {
       return g_qk(ctx, type, count(T), count(Hq), count(Hk), count(D), count(rotary), flags, q.p, q.token, q.head, k.p,
                   k.token, k.head, qo.p, qo.token, qo.head, ko.p, ko.token, ko.head, qw, kw, float(eps), table,
                   count(rows), positions, cu, count(seqs));
     });
+    if (code == AE_OK) {
+      written(tensor(args[4], "q_out"));
+      written(tensor(args[5], "k_out"));
+    }
+    return PyLong_FromLong(code);
   });
 }
 

@@ -52,3 +52,23 @@ def test_tensors_without_an_address_raise(call, args):
         one = [*args[:i], a.replace("Hollow", "batched"), *args[i + 1:]]
         lines += f"try:\n    m.{call}(0, 0, {', '.join(one)})\nexcept RuntimeError as e:\n    print('storage' in str(e))\n"
     assert run(lines).split() == ["True"] * sum("Hollow" in a for a in args)
+
+
+def test_gradients_are_not_dropped():
+    """The calls compute none: a float operand or result that requires one is refused while gradients are recorded, whichever
+    it is, and taken under no_grad."""
+    operands = {
+        "matmul_i8": ["Hollow(2, 8, dtype=i8)", "grad(2)", "Hollow(4, 8, dtype=i8)", "grad(4)", "grad(2, 4)", "grad(4)"],
+        "linear_i8": ["grad(2, 8)", "grad(8)", "Hollow(4, 8, dtype=i8)", "grad(4)", "grad(2, 4)", "grad(4)"],
+        "qk_norm_rope": ["grad(2, 3, 8)", "grad(2, 1, 8)", "grad(2, 3, 8)", "grad(2, 1, 8)", "grad(5, 4)",
+                         "Hollow(2, dtype=torch.int32)", "None", "grad(8)", "grad(8)", "1e-6", "0"]}
+    lines = "i8 = torch.int8\ndef grad(*size): return Hollow(*size).requires_grad_()\n"
+    count = 0
+    for call, args in operands.items():
+        for i, a in enumerate(args):
+            if "grad" in a:
+                one = [x.replace("grad", "Hollow") if j != i else x for j, x in enumerate(args)]
+                count += 1
+                lines += (f"args = [0, 0, {', '.join(one)}]\ntry:\n    m.{call}(*args)\nexcept ValueError as e:\n"
+                          f"    print('requires grad' in str(e))\nwith torch.no_grad():\n    assert m.{call}(*args) == -1\n")
+    assert run(lines).split() == ["True"] * count

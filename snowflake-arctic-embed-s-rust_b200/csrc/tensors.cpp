@@ -30,6 +30,7 @@ struct Refused {};  // a Python exception is set
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) refuse("%s must be a torch tensor%s", what);
   const at::Tensor& t = THPVariable_Unpack(o);
+  if (t.is_neg()) refuse("%s holds the negatives of its values: call resolve_neg() on it%s", what);
   // as torch refuses operations with out=: a gradient would end here without a word
   if (t.requires_grad() && c10::GradMode::is_enabled())
     refuse("%s requires grad, but no gradients are computed: call this under torch.no_grad()%s", what);

@@ -72,3 +72,19 @@ def test_gradients_are_not_dropped():
                 lines += (f"args = [0, 0, {', '.join(one)}]\ntry:\n    m.{call}(*args)\nexcept ValueError as e:\n"
                           f"    print('requires grad' in str(e))\nwith torch.no_grad():\n    assert m.{call}(*args) == -1\n")
     assert run(lines).split() == ["True"] * count
+
+
+def test_tensors_that_stand_for_their_negatives_are_refused():
+    """A lazily negated view (the imaginary part of a conjugate) holds the negatives of its values."""
+    import torch
+
+    from arctic_embed_s_int8 import _lib
+
+    z = torch.ones(4, 1, dtype=torch.complex64)
+    x = z.conj().imag
+    assert x.is_neg()
+    m, w = _lib.tensors(), torch.zeros(3, 1, dtype=torch.int8)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        m.linear_i8(0, 0, x, None, w, torch.zeros(3), torch.zeros(4, 3), None)
+    with pytest.raises(ValueError, match="device memory"):  # as it is refused for being on the host otherwise
+        m.linear_i8(0, 0, x.resolve_neg(), None, w, torch.zeros(3), torch.zeros(4, 3), None)

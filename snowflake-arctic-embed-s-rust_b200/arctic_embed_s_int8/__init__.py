@@ -198,14 +198,14 @@ class Engine:
         tensors: a [M, K] and w [N, K] int8, a_scale [M], w_scale [N] and bias [N] float32, out [M, N]
         float32, float16 or bfloat16. Rows may have any pitch. Asynchronous on the engine's stream. Computes no
         gradients (nor do linear_i8 and qk_norm_rope): tensors that require them are refused unless grad mode is off."""
-        code = tensors().matmul_i8(self._h.value, self.device, a, a_scale, w, w_scale, out, bias)
+        code = tensors().matmul_i8(self._h and self._h.value, self.device, a, a_scale, w, w_scale, out, bias)
         if code:
             self._check(code)
 
     def linear_i8(self, x, w, w_scale, out, bias=None, inv_smooth=None) -> None:
         """ae_linear_i8: the same product from float activations x [M, K] (float32, float16 or bfloat16),
         multiplied by inv_smooth [K] and quantized to int8 with a scale for each token on the way."""
-        code = tensors().linear_i8(self._h.value, self.device, x, inv_smooth, w, w_scale, out, bias)
+        code = tensors().linear_i8(self._h and self._h.value, self.device, x, inv_smooth, w, w_scale, out, bias)
         if code:
             self._check(code)
 
@@ -223,7 +223,7 @@ class Engine:
         may be q and k). table [rows, rotary] float32 is rope_table's; a token's position is positions[t]
         (int32), or its place in its sequence of cu (int32 or uint32 [n_seqs + 1])."""
         flags = (self.QK_NEIGHBOURS if neighbours else 0) | (0 if norm else self.QK_NO_NORM)
-        code = tensors().qk_norm_rope(self._h.value, self.device, q, k, q_out, k_out, table, positions, cu, q_weight,
+        code = tensors().qk_norm_rope(self._h and self._h.value, self.device, q, k, q_out, k_out, table, positions, cu, q_weight,
                                       k_weight, eps, flags)
         if code:
             self._check(code)

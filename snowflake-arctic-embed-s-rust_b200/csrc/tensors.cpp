@@ -112,7 +112,9 @@ uint64_t pitch(const at::Tensor& t) {
   return uint64_t(t.size(0) > 1 && t.size(1) ? t.stride(0) : t.size(1));
 }
 
+// None, a closed engine's, is the null context, which the C ABI refuses.
 ae_ctx* context(PyObject* o) {
+  if (o == Py_None) return nullptr;
   void* p = PyLong_AsVoidPtr(o);
   if (!p && PyErr_Occurred()) throw Refused{};
   return static_cast<ae_ctx*>(p);

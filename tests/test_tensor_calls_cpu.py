@@ -88,3 +88,20 @@ def test_tensors_that_stand_for_their_negatives_are_refused():
         m.linear_i8(0, 0, x, None, w, torch.zeros(3), torch.zeros(4, 3), None)
     with pytest.raises(ValueError, match="device memory"):  # as it is refused for being on the host otherwise
         m.linear_i8(0, 0, x.resolve_neg(), None, w, torch.zeros(3), torch.zeros(4, 3), None)
+
+
+def test_a_closed_engine_is_refused_as_everywhere():
+    """AeError, as the engine's other calls raise it."""
+    lines = """
+from arctic_embed_s_int8 import AeError, Engine
+e = Engine.__new__(Engine)
+e._h, e.device, i8 = None, 0, torch.int8
+h, w = Hollow(2, 1, 8), Hollow(4, 8, dtype=i8)
+for call in (lambda: e.sync(), lambda: e.matmul_i8(Hollow(2, 8, dtype=i8), Hollow(2), w, Hollow(4), Hollow(2, 4)),
+             lambda: e.linear_i8(Hollow(2, 8), w, Hollow(4), Hollow(2, 4)), lambda: e.qk_norm_rope(h, h, h, h)):
+    try:
+        call()
+    except AeError as x:
+        print(x.code)
+"""
+    assert run(lines).split() == ["-1"] * 4

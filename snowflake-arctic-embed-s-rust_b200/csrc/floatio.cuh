@@ -1,4 +1,4 @@
-// 16-byte pieces of float, half or bfloat16 rows, widened to and rounded from float.
+// 16-byte pieces of float, half or bfloat16 rows, widened to float, and roundings from it.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -63,13 +63,6 @@ __device__ __forceinline__ void widen(uint4 p, float (&v)[kPiece<T>]) {
       v[2 * i + 1] = f.y;
     }
   }
-}
-template <class T>
-__device__ __forceinline__ uint4 narrow(const float (&v)[kPiece<T>]) {
-  if constexpr (sizeof(T) == 4)
-    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  else
-    return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
 }  // namespace ae

@@ -180,8 +180,8 @@ enum { AE_F32 = 0, AE_F16 = 1, AE_BF16 = 2 };
  *   out[m, n] = fma(float(sum_k a[m, k] w[n, k]), a_scale[m] * w_scale[n], bias[n])
  * a [M, K], w [N, K] (out_features x in_features), a_scale [M], w_scale [N], bias [N] or NULL (zeros), out
  * [M, N] of out_type. The sum is exact (int32, hence K <= 131,071); the result is rounded to out_type once.
- * lda, ldw (bytes) and ldo (elements) are the rows' pitches, at least the rows' lengths. Any M (0: nothing
- * is done), N and K. Operands that start on 16 bytes with a pitch that is a multiple of 16 are read where
+ * lda, ldw (bytes) and ldo (elements) are the rows' pitches, at least the rows' lengths. M up to 2^30 (0: nothing
+ * is done), N 1 to 2^30. Operands that start on 16 bytes with a pitch that is a multiple of 16 are read where
  * they are; others are first laid out so in scratch (ae_release_scratch). out overlaps no operand. */
 int ae_matmul_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, const int8_t* d_a, uint64_t lda,
                  const float* d_a_scale, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
@@ -192,7 +192,7 @@ int ae_matmul_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, const int8_t* 
  *   y = x * inv_smooth (NULL: ones);  top = max_k |y|;  a = round_half_even(y * (127 / top));
  *   a_scale = top / 127
  * A token whose top is below 2^-119 (127 / top would not be finite) quantizes to zeros with a scale of 0;
- * one that holds an infinity or a NaN gives a row of NaN. */
+ * one whose y holds an infinity or a NaN gives a row of NaN. */
 int ae_linear_i8(ae_ctx* ctx, uint32_t M, uint32_t N, uint32_t K, int x_type, const void* d_x, uint64_t ldx,
                  const float* d_inv_smooth, const int8_t* d_w, uint64_t ldw, const float* d_w_scale,
                  const float* d_bias, int out_type, void* d_out, uint64_t ldo);

@@ -20,7 +20,7 @@
 //   SPLIT  a cluster of 2..8 CTAs splits the depth of one tile and adds the partial sums through distributed
 //          shared memory, where there are too few tiles for the SMs.
 // Device times and what bounds them: 16,384 x 8,192 x 4,096 to bfloat16 351 us (PAIR: 512 cycles a depth block, the
-// tensor pipe's rate, at the 1.3 GHz that the power cap leaves); 65,536 x 1,536 x 384 48 us (the epilogue, 3,200 cycles a
+// tensor pipe's rate, at the 1.3 GHz that the power cap leaves); 65,536 x 1,536 x 384 46-49 us (the epilogue, 3,200 cycles a
 // 256 x 256 tile against 1,536 of MMAs); 1 x 4,096 x 4,096 5 us, 1 x 18,944 x 4,096 16 us (the weights' bytes: 6.5 TB/s
 // beyond the first 4 us).
 #include <algorithm>
@@ -612,7 +612,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // --------------------------------------------------------------------------- operands as TMA reads them
-// Rows that do not start on 16 bytes are laid out at a pitch that does: 4 bytes a thread.
+// Rows that do not start on 16 bytes are laid out at a pitch that does: 4 bytes a thread, read one by one at any address.
+// Each call does so again: 4,096 x 4,095 weights take 12 us, bound by the issue of instructions (68 % of the slots, DRAM
+// 12 %); 1 x 4,096 x 4,095 to bfloat16 takes 18.4 us with them and 6.5 from rows of 4,096 bytes, 33 x 30,522 x 383 to
+// float 15.6 and 6.0.
 __global__ void __launch_bounds__(256) k_lay_rows(const int8_t* src, size_t ld, int rows, int K, uint32_t* dst,
                                                   int words) {
   pdl_wait();
@@ -802,7 +805,8 @@ size_t product_scratch(const ProductArgs& a) {
 
 // Up to 16 tokens whose depth (its share of a split) fits a CTA's token blocks, and little enough to read in each of
 // some 130 CTAs at once. On the device one 4,096-deep bfloat16 token takes 6.3 us this way and 6.7 us in two kernels,
-// two smoothed ones 7.3 and 6.8, sixteen 11.6 and 7.1; a launch less spares the host about 2 us.
+// two smoothed ones 7.3 and 6.8, sixteen 11.6 and 7.1. A launch less spares the host about 2 us, so up to the bound a
+// call that the host makes gains; one replayed from a graph loses up to 0.5 us near it.
 int launch_product_fused(const ProductArgs& args, const QuantArgs& q, cudaStream_t st) {
   ProductArgs a = args;
   if (a.M > 16 || size_t(a.M) * a.K * float_type_bytes(q.x_type) > kFuseMost || !in_place(a.w, a.ldw, a.N)) return 1;
